@@ -31,11 +31,15 @@ class DType(enum.IntEnum):
     """DType::code() wire values (tensor_view.rs:160-209)."""
     F32 = 0
     F16 = 1
+    Q4_0 = 2
+    Q4_1 = 3
+    Q4_K = 12
     I32 = 26
     I64 = 27
+    BF16 = 30
 
 
-DTYPE_SIZE = {DType.F32: 4, DType.F16: 2, DType.I32: 4, DType.I64: 8}
+DTYPE_SIZE = {DType.F32: 4, DType.F16: 2, DType.BF16: 2, DType.I32: 4, DType.I64: 8}
 
 
 class Status(enum.IntEnum):
@@ -164,6 +168,18 @@ class CFlashAttnOptions(ctypes.Structure):
         return o
 
 
+class CPagedAttnOptions(ctypes.Structure):
+    """emel_paged_attn_options."""
+    _fields_ = [("scale", ctypes.c_float), ("has_scale", ctypes.c_uint32), ("window", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32)]
+
+
+class CQ4Weights(ctypes.Structure):
+    """emel_q4_weights."""
+    _fields_ = [("data", ctypes.c_void_p), ("bytes", ctypes.c_uint64), ("k", ctypes.c_uint64),
+                ("rows", ctypes.c_uint64), ("dtype", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+
 # Every symbol include/emel_cuda.h declares, with its ctypes signature.
 _P = ctypes.POINTER(CView)
 _V = ctypes.c_void_p
@@ -240,6 +256,13 @@ SIGNATURES = {
     "emel_cuda_cpy": (_I, [_CTX, _V, _P, _P]),
     "emel_cuda_cont": (_I, [_CTX, _V, _P, _P]),
     "emel_cuda_glu": (_I, [_CTX, _V, _I, _V, ctypes.c_uint64, _V, ctypes.c_uint64]),
+    "emel_cuda_paged_kv_append": (_I, [_CTX, _V, _P, _P, _P, _P, _P, _P, _P]),
+    "emel_cuda_paged_attn": (_I, [_CTX, _V, _P, _P, _P, _P, _P, _P, ctypes.POINTER(CPagedAttnOptions)]),
+    "emel_cuda_q4_packed_bytes": (_I, [ctypes.c_uint32, ctypes.c_uint64, ctypes.c_uint64,
+                                       ctypes.POINTER(ctypes.c_uint64)]),
+    "emel_cuda_q4_pack": (_I, [_CTX, _V, _P, _V, ctypes.c_uint64, ctypes.POINTER(CQ4Weights)]),
+    "emel_cuda_mul_mat_q4": (_I, [_CTX, _V, ctypes.POINTER(CQ4Weights), _P, _P]),
+    "emel_cuda_logits_adjust": (_I, [_CTX, _V, _P, _P, _P, _P, _P, _P, _P]),
     "emel_cuda_exchange_create": (_I, [_CTX, _I, _I, ctypes.c_uint32, ctypes.c_uint32, ctypes.POINTER(_V)]),
     "emel_cuda_exchange_handle": (_I, [_V, _V]),
     "emel_cuda_exchange_connect": (_I, [_CTX, _V, _V]),
@@ -1040,6 +1063,103 @@ class OpGlu(Event):
         (ip, il), (op, ol) = self.input, self.output
         return ctx._lib.emel_cuda_glu(ctx.handle, stream, int(self.subop), ctypes.c_void_p(ip), il,
                                       ctypes.c_void_p(op), ol)
+
+
+# ---------------------------------------------------------------------------
+# One decoding step: paged cache, its attention, 4-bit projections, logits
+# ---------------------------------------------------------------------------
+
+@dataclass
+class OpPagedKvAppend(Event):
+    """New keys and values [d, kv_heads, count] into the pages of a cache
+    [d, kv_heads, page_size, pages] (emel_cuda_paged_kv_append): row i goes to
+    position positions[i] of sequence sequences[i] (None: of sequence i)."""
+    key: TensorView
+    value: TensorView
+    block_table: TensorView
+    sequences: Optional[TensorView]
+    positions: TensorView
+    key_cache: TensorView
+    value_cache: TensorView
+
+    def dispatch(self, ctx, stream):
+        return ctx._lib.emel_cuda_paged_kv_append(ctx.handle, stream, _r(self.key), _r(self.value),
+                                                  _r(self.block_table), _r(self.sequences), _r(self.positions),
+                                                  _r(self.key_cache), _r(self.value_cache))
+
+
+@dataclass
+class OpPagedAttn(Event):
+    """One new token of every sequence, query / destination [d, heads, batch],
+    over its cached tokens (emel_cuda_paged_attn).  scale: None for
+    1 / sqrt(d); window: how many of the last tokens are seen, 0 for all."""
+    query: TensorView
+    key_cache: TensorView
+    value_cache: TensorView
+    block_table: TensorView
+    lengths: TensorView
+    destination: TensorView
+    scale: Optional[float] = None
+    window: int = 0
+
+    def dispatch(self, ctx, stream):
+        opts = CPagedAttnOptions(self.scale or 0.0, self.scale is not None, self.window, 0)
+        return ctx._lib.emel_cuda_paged_attn(ctx.handle, stream, _r(self.query), _r(self.key_cache),
+                                             _r(self.value_cache), _r(self.block_table), _r(self.lengths),
+                                             _r(self.destination), ctypes.byref(opts))
+
+
+class Q4Weights:
+    """Rows of Q4_0, Q4_1 or Q4_K blocks laid out once for OpMulMatQ4
+    (emel_cuda_q4_pack) in a device buffer of the library.  `source`, a block
+    view [k, rows] such as GgufImage.upload returns, is not needed after the
+    layout has run on `stream`."""
+
+    def __init__(self, ctx: "Context", source, stream=None):
+        view = source if isinstance(source, CView) else source.c()
+        need = ctypes.c_uint64()
+        _check(ctx._lib.emel_cuda_q4_packed_bytes(view.dtype, view.ne[0], view.ne[1], ctypes.byref(need)),
+               "q4_packed_bytes")
+        self.buffer = DeviceBuffer(ctx, need.value)
+        self.c = CQ4Weights()
+        _check(ctx._lib.emel_cuda_q4_pack(ctx.handle, stream, ctypes.byref(view), ctypes.c_void_p(self.buffer.ptr),
+                                          need.value, ctypes.byref(self.c)), "q4_pack")
+
+    def free(self):
+        self.buffer.free()
+
+
+@dataclass
+class OpMulMatQ4(Event):
+    """destination [rows, n] = weights [k, rows] times rhs [k, n], for one or a
+    few columns n (emel_cuda_mul_mat_q4)."""
+    weights: Q4Weights
+    rhs: TensorView
+    destination: TensorView
+
+    def dispatch(self, ctx, stream):
+        return ctx._lib.emel_cuda_mul_mat_q4(ctx.handle, stream, ctypes.byref(self.weights.c), _r(self.rhs),
+                                             _r(self.destination))
+
+
+@dataclass
+class OpLogitsAdjust(Event):
+    """Penalties for repeated tokens, biases and the mask of allowed tokens on
+    logits [vocab, rows] (emel_cuda_logits_adjust).  history, history_lengths
+    and penalties (repetition, frequency, presence) come together or not at
+    all."""
+    src: TensorView
+    dst: TensorView
+    history: Optional[TensorView] = None
+    history_lengths: Optional[TensorView] = None
+    penalties: Optional[TensorView] = None
+    bias: Optional[TensorView] = None
+    allowed: Optional[TensorView] = None
+
+    def dispatch(self, ctx, stream):
+        return ctx._lib.emel_cuda_logits_adjust(ctx.handle, stream, _r(self.src), _r(self.history),
+                                                _r(self.history_lengths), _r(self.penalties), _r(self.bias),
+                                                _r(self.allowed), _r(self.dst))
 
 
 class Kernel:

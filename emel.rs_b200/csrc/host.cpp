@@ -39,6 +39,7 @@ uint64_t dtype_size(uint32_t dtype) {
     switch (dtype) {
     case EMEL_DTYPE_F32: return 4;
     case EMEL_DTYPE_F16: return 2;
+    case EMEL_DTYPE_BF16: return 2;
     case EMEL_DTYPE_I32: return 4;
     case EMEL_DTYPE_I64: return 8;
     default: return 0;
@@ -1691,6 +1692,303 @@ emel_cuda_status emel_cuda_soft_max_diag_mask_inf(emel_cuda_context* ctx, void* 
         input_len > UINT64_MAX / 8 || (input != output && ranges_overlap(input, input_len * 4, output, output_len * 4)))
         return EMEL_CUDA_INVALID_ARGUMENT;
     return diag_launch(ctx, stream, input, output, side, (uint64_t)n_past, emel::kDiagSoftMaxCausal);
+}
+
+// ---- one decoding step: paged cache, 4-bit projections, logits -----------------
+
+// dimension 0 adjacent in memory
+static bool unit_rows(const emel_tensor_view* v, const Checked& c) { return v->ne[0] == 1 || c.nb[0] == c.elem; }
+
+// The bytes between a view's first and last element.
+static uint64_t reach_of(const emel_tensor_view* v, const Checked& c) {
+    uint64_t n = c.elem;
+    for (int d = 0; d < 4; ++d) n += (v->ne[d] - 1) * c.nb[d];
+    return n;
+}
+
+static bool views_overlap(const emel_tensor_view* a, const Checked& ca, const emel_tensor_view* b, const Checked& cb) {
+    return ranges_overlap(a->data, reach_of(a, ca), b->data, reach_of(b, cb));
+}
+
+static uint32_t* reject_word(emel_cuda_context* ctx) {
+    return reinterpret_cast<uint32_t*>(static_cast<char*>(ctx->workspace) + emel::kRejectWordOffset);
+}
+
+// The cache's views and its table: shared by the append and the attention.
+static emel_cuda_status paged_cache_valid(const emel_tensor_view* k, const emel_tensor_view* v,
+                                          const emel_tensor_view* table, Checked* ck, Checked* cv, Checked* ct) {
+    if (k == nullptr || v == nullptr || (k->dtype != EMEL_DTYPE_F16 && k->dtype != EMEL_DTYPE_BF16) ||
+        !validate_as(k, k->dtype, false, ck) || !validate_as(v, k->dtype, false, cv) ||
+        !validate_as(table, EMEL_DTYPE_I32, false, ct))
+        return EMEL_CUDA_INVALID_VIEW;
+    if (!unit_rows(k, *ck) || !unit_rows(v, *cv)) return EMEL_CUDA_INVALID_LAYOUT;
+    if (!same_ne(k, v) || k->ne[0] > (uint64_t)emel::kPagedMaxD || k->ne[2] > 0x7fffffffull ||
+        k->ne[3] > 0x7fffffffull || table->ne[2] != 1 || table->ne[3] != 1 || table->ne[0] > 0x7fffffffull ||
+        table->ne[1] > 0x7fffffffull)
+        return EMEL_CUDA_SHAPE_MISMATCH;
+    return EMEL_CUDA_OK;
+}
+
+static bool vector_shape(const emel_tensor_view* v, uint64_t n) {
+    return v->ne[0] == n && v->ne[1] == 1 && v->ne[2] == 1 && v->ne[3] == 1;
+}
+
+emel_cuda_status emel_cuda_paged_kv_append(emel_cuda_context* ctx, void* stream, const emel_tensor_view* key,
+                                           const emel_tensor_view* value, const emel_tensor_view* block_table,
+                                           const emel_tensor_view* sequences, const emel_tensor_view* positions,
+                                           const emel_tensor_view* key_cache, const emel_tensor_view* value_cache) {
+    Checked ck, cv, ct, cn, cw, cs, cp;
+    emel_cuda_status st = paged_cache_valid(key_cache, value_cache, block_table, &ck, &cv, &ct);
+    if (st == EMEL_CUDA_INVALID_VIEW) return st;
+    if (key == nullptr || value == nullptr || (key->dtype != EMEL_DTYPE_F32 && key->dtype != key_cache->dtype) ||
+        !validate_as(key, key->dtype, false, &cn) || !validate_as(value, key->dtype, false, &cw) ||
+        (sequences != nullptr && !validate_as(sequences, EMEL_DTYPE_I32, false, &cs)) ||
+        !validate_as(positions, EMEL_DTYPE_I32, false, &cp))
+        return EMEL_CUDA_INVALID_VIEW;
+    if (st != EMEL_CUDA_OK) return st;
+    if (!unit_rows(key, cn) || !unit_rows(value, cw)) return EMEL_CUDA_INVALID_LAYOUT;
+    const uint64_t count = key->ne[2];
+    if (!same_ne(key, value) || key->ne[0] != key_cache->ne[0] || key->ne[1] != key_cache->ne[1] || key->ne[3] != 1 ||
+        !vector_shape(positions, count) ||
+        (sequences != nullptr ? !vector_shape(sequences, count) : block_table->ne[1] != count))
+        return EMEL_CUDA_SHAPE_MISMATCH;
+    if (ctx == nullptr) return EMEL_CUDA_INVALID_ARGUMENT;
+    emel::PagedAppendPlan p{};
+    p.key = static_cast<const char*>(key->data);
+    p.value = static_cast<const char*>(value->data);
+    for (int d = 0; d < 3; ++d) {
+        p.key_st[d] = cn.nb[d];
+        p.value_st[d] = cw.nb[d];
+    }
+    p.table = static_cast<const int32_t*>(block_table->data);
+    for (int d = 0; d < 2; ++d) p.table_st[d] = (int64_t)(ct.nb[d] / 4);
+    p.table_pages = block_table->ne[0];
+    p.sequences_count = block_table->ne[1];
+    if (sequences != nullptr) {
+        p.sequences = static_cast<const int32_t*>(sequences->data);
+        p.seq_st = (int64_t)(cs.nb[0] / 4);
+    }
+    p.positions = static_cast<const int32_t*>(positions->data);
+    p.pos_st = (int64_t)(cp.nb[0] / 4);
+    p.k_cache = static_cast<char*>(key_cache->data);
+    p.v_cache = static_cast<char*>(value_cache->data);
+    for (int d = 0; d < 4; ++d) {
+        p.k_st[d] = ck.nb[d];
+        p.v_st[d] = cv.nb[d];
+    }
+    p.d = key_cache->ne[0];
+    p.kv_heads = key_cache->ne[1];
+    p.count = count;
+    p.page_size = key_cache->ne[2];
+    p.pages = key_cache->ne[3];
+    p.src_f32 = key->dtype == EMEL_DTYPE_F32;
+    p.cache_bf16 = key_cache->dtype == EMEL_DTYPE_BF16;
+    p.reject = reject_word(ctx);
+    p.reject_code = EMEL_CUDA_INDEX_OUT_OF_BOUNDS;
+    cudaError_t err = select_device(ctx);
+    if (err == cudaSuccess) err = emel::launch_paged_append(env_of(ctx, stream), p);
+    return device_status(ctx, err);
+}
+
+emel_cuda_status emel_cuda_paged_attn(emel_cuda_context* ctx, void* stream, const emel_tensor_view* query,
+                                      const emel_tensor_view* key_cache, const emel_tensor_view* value_cache,
+                                      const emel_tensor_view* block_table, const emel_tensor_view* lengths,
+                                      const emel_tensor_view* dst, const emel_paged_attn_options* options) {
+    Checked ck, cv, ct, cq, cl, cd;
+    emel_cuda_status st = paged_cache_valid(key_cache, value_cache, block_table, &ck, &cv, &ct);
+    if (st == EMEL_CUDA_INVALID_VIEW) return st;
+    if (query == nullptr || dst == nullptr || (query->dtype != EMEL_DTYPE_F32 && query->dtype != key_cache->dtype) ||
+        !validate_as(query, query->dtype, false, &cq) || !validate_as(lengths, EMEL_DTYPE_I32, false, &cl) ||
+        !validate_as(dst, query->dtype, false, &cd))
+        return EMEL_CUDA_INVALID_VIEW;
+    if (st != EMEL_CUDA_OK) return st;
+    if (!unit_rows(query, cq) || !unit_rows(dst, cd)) return EMEL_CUDA_INVALID_LAYOUT;
+    const uint64_t d = key_cache->ne[0], kv_heads = key_cache->ne[1], heads = query->ne[1], batch = query->ne[2];
+    if (!same_ne(query, dst) || query->ne[0] != d || query->ne[3] != 1 || heads % kv_heads != 0 ||
+        heads > 0x7fffffffull || block_table->ne[1] != batch || !vector_shape(lengths, batch))
+        return EMEL_CUDA_SHAPE_MISMATCH;
+    float scale = 1.0f / std::sqrt((float)d);
+    if (options != nullptr && options->has_scale) scale = options->scale;
+    if (!std::isfinite(scale) || !(scale > 0.0f) || (options != nullptr && options->reserved != 0))
+        return EMEL_CUDA_INVALID_PARAMETERS;
+    if (ctx == nullptr || views_overlap(dst, cd, query, cq) || views_overlap(dst, cd, key_cache, ck) ||
+        views_overlap(dst, cd, value_cache, cv) || views_overlap(dst, cd, block_table, ct) ||
+        views_overlap(dst, cd, lengths, cl))
+        return EMEL_CUDA_INVALID_ARGUMENT;
+    emel::PagedAttnPlan p{};
+    p.q = static_cast<const char*>(query->data);
+    p.dst = static_cast<char*>(dst->data);
+    for (int i = 0; i < 3; ++i) {
+        p.q_st[i] = cq.nb[i];
+        p.dst_st[i] = cd.nb[i];
+    }
+    p.k = static_cast<const char*>(key_cache->data);
+    p.v = static_cast<const char*>(value_cache->data);
+    for (int i = 0; i < 4; ++i) {
+        p.k_st[i] = ck.nb[i];
+        p.v_st[i] = cv.nb[i];
+    }
+    p.table = static_cast<const int32_t*>(block_table->data);
+    for (int i = 0; i < 2; ++i) p.table_st[i] = (int64_t)(ct.nb[i] / 4);
+    p.table_pages = block_table->ne[0];
+    p.lengths = static_cast<const int32_t*>(lengths->data);
+    p.len_st = (int64_t)(cl.nb[0] / 4);
+    p.d = d;
+    p.heads = heads;
+    p.batch = batch;
+    p.rep = heads / kv_heads;
+    p.page_size = key_cache->ne[2];
+    p.pages = key_cache->ne[3];
+    p.window = options != nullptr ? options->window : 0;
+    p.scale = scale;
+    p.q_f32 = query->dtype == EMEL_DTYPE_F32;
+    p.cache_bf16 = key_cache->dtype == EMEL_DTYPE_BF16;
+    p.reject = reject_word(ctx);
+    p.reject_code = EMEL_CUDA_INDEX_OUT_OF_BOUNDS;
+    cudaError_t err = select_device(ctx);
+    if (err == cudaSuccess) err = emel::launch_paged_attn(env_of(ctx, stream), p);
+    return device_status(ctx, err);
+}
+
+static bool q4_block(uint32_t dtype, uint64_t* values, uint64_t* bytes) {
+    *values = dtype == EMEL_DTYPE_Q4_K ? 256 : 32;
+    *bytes = dtype == EMEL_DTYPE_Q4_K ? 144 : dtype == EMEL_DTYPE_Q4_1 ? 20 : 18;
+    return dtype == EMEL_DTYPE_Q4_0 || dtype == EMEL_DTYPE_Q4_1 || dtype == EMEL_DTYPE_Q4_K;
+}
+
+emel_cuda_status emel_cuda_q4_packed_bytes(uint32_t dtype, uint64_t k, uint64_t rows, uint64_t* bytes) {
+    uint64_t values = 0, size = 0;
+    if (bytes == nullptr || !q4_block(dtype, &values, &size) || k == 0 || rows == 0 || k % values != 0 ||
+        !emel::q4_packed_bytes((int)dtype, k, rows, bytes))
+        return EMEL_CUDA_INVALID_ARGUMENT;
+    return EMEL_CUDA_OK;
+}
+
+emel_cuda_status emel_cuda_q4_pack(emel_cuda_context* ctx, void* stream, const emel_tensor_view* src, void* data,
+                                   uint64_t bytes, emel_q4_weights* out) {
+    uint64_t values = 0, size = 0, row_bytes = 0, need = 0;
+    if (src == nullptr || !q4_block(src->dtype, &values, &size) ||
+        !gr_packed_view_valid(src, src->dtype, values, size, &row_bytes))
+        return EMEL_CUDA_INVALID_VIEW;
+    if (src->ne[2] != 1 || src->ne[3] != 1) return EMEL_CUDA_SHAPE_MISMATCH;
+    if (emel_cuda_q4_packed_bytes(src->dtype, src->ne[0], src->ne[1], &need) != EMEL_CUDA_OK || bytes < need)
+        return EMEL_CUDA_CAPACITY;
+    if (ctx == nullptr || out == nullptr || data == nullptr || !aligned16(data) ||
+        ranges_overlap(data, need, src->data, row_bytes * src->ne[1]))
+        return EMEL_CUDA_INVALID_ARGUMENT;
+    emel::Q4PackPlan p{};
+    p.src = static_cast<const uint8_t*>(src->data);
+    p.dst = static_cast<uint8_t*>(data);
+    p.k = src->ne[0];
+    p.rows = src->ne[1];
+    p.row_bytes = row_bytes;
+    p.code = (int)src->dtype;
+    cudaError_t err = select_device(ctx);
+    if (err == cudaSuccess) err = emel::launch_q4_pack(env_of(ctx, stream), p);
+    if (err == cudaSuccess) *out = emel_q4_weights{data, need, p.k, p.rows, src->dtype, 0};
+    return device_status(ctx, err);
+}
+
+emel_cuda_status emel_cuda_mul_mat_q4(emel_cuda_context* ctx, void* stream, const emel_q4_weights* weights,
+                                      const emel_tensor_view* rhs, const emel_tensor_view* dst) {
+    Checked cr, cd;
+    uint64_t need = 0;
+    if (weights == nullptr || weights->data == nullptr || !aligned16(weights->data) || weights->reserved != 0 ||
+        emel_cuda_q4_packed_bytes(weights->dtype, weights->k, weights->rows, &need) != EMEL_CUDA_OK ||
+        weights->bytes < need || !validate_float(rhs, false, &cr) || !validate_float(dst, false, &cd))
+        return EMEL_CUDA_INVALID_VIEW;
+    if (!unit_rows(rhs, cr) || !unit_rows(dst, cd)) return EMEL_CUDA_INVALID_LAYOUT;
+    const uint64_t n = rhs->ne[1];
+    if (rhs->ne[0] != weights->k || rhs->ne[2] != 1 || rhs->ne[3] != 1 || dst->ne[0] != weights->rows ||
+        dst->ne[1] != n || dst->ne[2] != 1 || dst->ne[3] != 1)
+        return EMEL_CUDA_SHAPE_MISMATCH;
+    if (ctx == nullptr || views_overlap(dst, cd, rhs, cr) ||
+        ranges_overlap(weights->data, need, dst->data, reach_of(dst, cd)))
+        return EMEL_CUDA_INVALID_ARGUMENT;
+    emel::Q4MatvecPlan p{};
+    p.weights = static_cast<const uint8_t*>(weights->data);
+    p.x = static_cast<const char*>(rhs->data);
+    p.dst = static_cast<char*>(dst->data);
+    p.k = weights->k;
+    p.rows = weights->rows;
+    p.n = n;
+    p.x_st = cr.nb[1];
+    p.dst_st = cd.nb[1];
+    p.code = (int)weights->dtype;
+    p.x_f16 = rhs->dtype == EMEL_DTYPE_F16;
+    p.dst_f16 = dst->dtype == EMEL_DTYPE_F16;
+    cudaError_t err = select_device(ctx);
+    if (err == cudaSuccess) err = emel::launch_mul_mat_q4(env_of(ctx, stream), p);
+    return device_status(ctx, err);
+}
+
+emel_cuda_status emel_cuda_logits_adjust(emel_cuda_context* ctx, void* stream, const emel_tensor_view* src,
+                                         const emel_tensor_view* history, const emel_tensor_view* history_lengths,
+                                         const emel_tensor_view* penalties, const emel_tensor_view* bias,
+                                         const emel_tensor_view* allowed, const emel_tensor_view* dst) {
+    Checked cs, cd, ch, cl, cp, cb, ca;
+    const bool past = history != nullptr;
+    if (!validate_float(src, false, &cs) || !validate_as(dst, src->dtype, false, &cd) ||
+        past != (history_lengths != nullptr) || past != (penalties != nullptr) ||
+        (past && (!validate_as(history, EMEL_DTYPE_I32, false, &ch) ||
+                  !validate_as(history_lengths, EMEL_DTYPE_I32, false, &cl) ||
+                  !validate_as(penalties, EMEL_DTYPE_F32, false, &cp))) ||
+        (bias != nullptr && !validate_as(bias, EMEL_DTYPE_F32, false, &cb)) ||
+        (allowed != nullptr && !validate_as(allowed, EMEL_DTYPE_I32, false, &ca)))
+        return EMEL_CUDA_INVALID_VIEW;
+    if (!unit_rows(src, cs) || !unit_rows(dst, cd) || (bias != nullptr && !unit_rows(bias, cb)) ||
+        (allowed != nullptr && !unit_rows(allowed, ca)))
+        return EMEL_CUDA_INVALID_LAYOUT;
+    const uint64_t vocab = src->ne[0], rows = src->ne[1], words = vocab / 32 + (vocab % 32 != 0);
+    auto table = [&](const emel_tensor_view* v, uint64_t cols, bool shared_ok) {
+        return v->ne[0] == cols && (v->ne[1] == rows || (shared_ok && v->ne[1] == 1)) && v->ne[2] == 1 && v->ne[3] == 1;
+    };
+    if (!same_ne(src, dst) || src->ne[2] != 1 || src->ne[3] != 1 ||
+        (past && (!table(history, history->ne[0], false) || !vector_shape(history_lengths, rows) ||
+                  !table(penalties, 3, true))) ||
+        (bias != nullptr && !table(bias, vocab, true)) || (allowed != nullptr && !table(allowed, words, true)))
+        return EMEL_CUDA_SHAPE_MISMATCH;
+    const bool in_place = src->data == dst->data && (rows == 1 || cs.nb[1] == cd.nb[1]);
+    if (ctx == nullptr || (!in_place && views_overlap(dst, cd, src, cs)) ||
+        (past && (views_overlap(dst, cd, history, ch) || views_overlap(dst, cd, history_lengths, cl) ||
+                  views_overlap(dst, cd, penalties, cp))) ||
+        (bias != nullptr && views_overlap(dst, cd, bias, cb)) ||
+        (allowed != nullptr && views_overlap(dst, cd, allowed, ca)) ||
+        emel::logits_blocks(vocab, rows) > 0x7fffffffull)
+        return EMEL_CUDA_INVALID_ARGUMENT;
+    emel::LogitsPlan p{};
+    p.src = static_cast<const char*>(src->data);
+    p.dst = static_cast<char*>(dst->data);
+    p.vocab = vocab;
+    p.rows = rows;
+    p.src_st = cs.nb[1];
+    p.dst_st = cd.nb[1];
+    if (past) {
+        p.history = static_cast<const int32_t*>(history->data);
+        p.history_len = history->ne[0];
+        p.lengths = static_cast<const int32_t*>(history_lengths->data);
+        p.len_st = (int64_t)(cl.nb[0] / 4);
+        p.penalties = static_cast<const float*>(penalties->data);
+        for (int i = 0; i < 2; ++i) {
+            p.hist_st[i] = (int64_t)(ch.nb[i] / 4);
+            p.pen_st[i] = (int64_t)(cp.nb[i] / 4);
+        }
+        p.penalty_rows = penalties->ne[1] != 1;
+    }
+    if (bias != nullptr) {
+        p.bias = static_cast<const float*>(bias->data);
+        p.bias_st = (int64_t)(cb.nb[1] / 4);
+        p.bias_rows = bias->ne[1] != 1;
+    }
+    if (allowed != nullptr) {
+        p.allowed = static_cast<const uint32_t*>(allowed->data);
+        p.allowed_st = (int64_t)(ca.nb[1] / 4);
+        p.allowed_rows = allowed->ne[1] != 1;
+    }
+    p.f16 = src->dtype == EMEL_DTYPE_F16;
+    cudaError_t err = select_device(ctx);
+    if (err == cudaSuccess) err = emel::launch_logits_adjust(env_of(ctx, stream), p);
+    return device_status(ctx, err);
 }
 
 // ---- gated linear units ------------------------------------------------------

@@ -206,6 +206,102 @@ struct DiagPlan {
 
 cudaError_t launch_diag(const LaunchEnv& env, const DiagPlan& plan, int mode);
 
+// Paged key/value cache (paged.cu).  Caches are [d, kv_heads, page_size,
+// pages] with byte strides; the block table is [pages of a sequence, sequence].
+constexpr int kPagedMaxD = 256;
+
+struct PagedAppendPlan {
+    const char* key;        // [d, kv_heads, count], byte strides, unit element stride in dim 0
+    const char* value;
+    uint64_t key_st[3], value_st[3];
+    const int32_t* table;
+    int64_t table_st[2];    // elements
+    uint64_t table_pages, sequences_count;
+    const int32_t* sequences;  // null: new row i belongs to sequence i
+    int64_t seq_st;
+    const int32_t* positions;
+    int64_t pos_st;
+    char* k_cache;
+    char* v_cache;
+    uint64_t k_st[4], v_st[4];
+    uint64_t d, kv_heads, count, page_size, pages;
+    bool src_f32, cache_bf16;
+    uint32_t* reject;
+    uint32_t reject_code;
+};
+
+cudaError_t launch_paged_append(const LaunchEnv& env, const PagedAppendPlan& plan);
+
+struct PagedAttnPlan {
+    const char* q;          // [d, heads, batch]
+    char* dst;
+    uint64_t q_st[3], dst_st[3];
+    const char* k;
+    const char* v;
+    uint64_t k_st[4], v_st[4];
+    const int32_t* table;
+    int64_t table_st[2];
+    uint64_t table_pages;
+    const int32_t* lengths;
+    int64_t len_st;
+    uint64_t d, heads, batch, rep, page_size, pages;
+    uint64_t window;        // 0: every cached token is seen
+    float scale;
+    bool q_f32, cache_bf16;
+    uint32_t* reject;
+    uint32_t reject_code;
+};
+
+cudaError_t launch_paged_attn(const LaunchEnv& env, const PagedAttnPlan& plan);
+
+// Matrix-vector products with 4-bit weights (q4.cu); code: the rows' dtype.
+struct Q4PackPlan {
+    const uint8_t* src;     // rows of k / 32 or k / 256 blocks
+    uint8_t* dst;           // packed layout, 16-byte aligned
+    uint64_t k, rows, row_bytes;
+    int code;
+};
+
+struct Q4MatvecPlan {
+    const uint8_t* weights;  // packed layout
+    const char* x;           // [k, n], binary32 or binary16, rows x_st bytes apart
+    char* dst;               // [rows, n], binary32 or binary16, rows dst_st bytes apart
+    uint64_t k, rows, n, x_st, dst_st;
+    int code;
+    bool x_f16, dst_f16;
+};
+
+bool q4_packed_bytes(int code, uint64_t k, uint64_t rows, uint64_t* bytes);
+cudaError_t launch_q4_pack(const LaunchEnv& env, const Q4PackPlan& plan);
+cudaError_t launch_mul_mat_q4(const LaunchEnv& env, const Q4MatvecPlan& plan);
+
+// Penalties, biases and masks on logits (logits.cu); strides in bytes for
+// src / dst, in elements for the rest.
+struct LogitsPlan {
+    const char* src;
+    char* dst;
+    uint64_t vocab, rows, src_st, dst_st;
+    const int32_t* history;  // null: no penalties
+    int64_t hist_st[2];
+    uint64_t history_len;
+    const int32_t* lengths;
+    int64_t len_st;
+    const float* penalties;
+    int64_t pen_st[2];
+    bool penalty_rows;       // one triple per row (else one for all)
+    const float* bias;       // null: none
+    int64_t bias_st;
+    bool bias_rows;
+    const uint32_t* allowed;  // null: every token
+    int64_t allowed_st;
+    bool allowed_rows;
+    bool f16;
+};
+
+// Blocks of one launch (at most 2^31 - 1 are possible).
+uint64_t logits_blocks(uint64_t vocab, uint64_t rows);
+cudaError_t launch_logits_adjust(const LaunchEnv& env, const LogitsPlan& plan);
+
 // Peer exchange over NVLink (exchange.cu).  Every rank owns one buffer of
 // kExchangeHeaderBytes flag words (flag r = the last epoch rank r published
 // into this buffer) followed by two banks (epoch parity) of kExchangeMaxRanks

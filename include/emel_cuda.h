@@ -743,6 +743,127 @@ EMEL_CUDA_API emel_cuda_status emel_gguf_upload(emel_cuda_context* ctx, void* st
                                                 uint64_t image_bytes, const emel_gguf_tensor_info* tensor,
                                                 void* device_dst, uint64_t device_bytes, emel_tensor_view* view_out);
 
+/* ---- one decoding step: paged cache, its attention, 4-bit projections -- */
+/* Operators of a serving step that the reference does not have; their parity
+ * is defined by the formulas below.  All views keep the layout rules of the
+ * other entry points; dimension 0 has unit stride where the text says "unit
+ * rows" (else EMEL_CUDA_INVALID_LAYOUT), every other dimension any stride.
+ * Work on the device, stream-ordered and graph-capturable; a captured step
+ * reads lengths, positions and tables when it is replayed.
+ *
+ * Paged key/value cache: key_cache and value_cache are [d, kv_heads,
+ * page_size, pages], F16 or BF16 (both the same), unit rows, d <= 256; the
+ * other strides decide whether pages are stored token by token or head by
+ * head.  block_table is I32 [pages of a sequence, sequences]: entry j of a
+ * column is the page that holds positions j * page_size ... of that sequence.
+ * Entries beyond a sequence's tokens are never read.  A page number outside
+ * [0, pages) or a position outside the table is found on the device: it is
+ * never used as an address, and the next emel_cuda_stream_synchronize returns
+ * EMEL_CUDA_INDEX_OUT_OF_BOUNDS. */
+
+/* Writes `count` new keys and values into their pages: key and value are
+ * [d, kv_heads, count], F32 or the cache's type, unit rows.  New row i goes to
+ * position positions[i] (I32 [count]) of sequence sequences[i] (I32 [count];
+ * NULL: of sequence i, and count is the table's number of sequences).  A
+ * negative position skips its row, a rejected one writes nothing; F32 is
+ * rounded once, to nearest even.  No two rows may name the same position of
+ * one sequence.
+ * Statuses: INVALID_VIEW, INVALID_LAYOUT, SHAPE_MISMATCH, INVALID_ARGUMENT
+ * (null context). */
+EMEL_CUDA_API emel_cuda_status emel_cuda_paged_kv_append(emel_cuda_context* ctx, void* stream,
+                                                         const emel_tensor_view* key, const emel_tensor_view* value,
+                                                         const emel_tensor_view* block_table,
+                                                         const emel_tensor_view* sequences,
+                                                         const emel_tensor_view* positions,
+                                                         const emel_tensor_view* key_cache,
+                                                         const emel_tensor_view* value_cache);
+
+/* Attention of one new token of every sequence over its cached tokens.
+ * query and dst are [d, heads, batch], F32 or the cache's type (both the
+ * same), unit rows; heads is a multiple of kv_heads, and query head h reads
+ * key/value head h / (heads / kv_heads); lengths is I32 [batch].  With
+ * n = lengths[b] and t over [window ? max(0, n - window) : 0, n):
+ *     s_t = scale * q . k_t,   dst = sum exp(s_t - max s) v_t / sum exp(s_t - max s)
+ * A sequence without tokens (n <= 0) gives zeros, and so does one whose every
+ * score is -inf.  Whatever lies in the cache beyond the n tokens (or before
+ * the window) has no effect, NaN and infinities included.  Scores, weights'
+ * sums and products are binary32; 16-bit queries round the weights to the
+ * cache's type before they meet the values.  A length beyond the table
+ * is taken as the table's and rejected (see above); tokens of a rejected page
+ * are left out.  dst may not overlap an input.
+ * options NULL: scale 1 / sqrt(d), no window.
+ * Statuses: INVALID_VIEW, INVALID_LAYOUT, SHAPE_MISMATCH, INVALID_PARAMETERS
+ * (scale not finite or not positive), INVALID_ARGUMENT (null context, an
+ * overlapping dst).  Uses the context's workspace: calls of one
+ * context must not overlap on the GPU. */
+typedef struct emel_paged_attn_options {
+    float scale;
+    uint32_t has_scale;
+    uint32_t window;   /* 0: none */
+    uint32_t reserved; /* must be 0 */
+} emel_paged_attn_options;
+EMEL_CUDA_API emel_cuda_status emel_cuda_paged_attn(emel_cuda_context* ctx, void* stream,
+                                                    const emel_tensor_view* query, const emel_tensor_view* key_cache,
+                                                    const emel_tensor_view* value_cache,
+                                                    const emel_tensor_view* block_table,
+                                                    const emel_tensor_view* lengths, const emel_tensor_view* dst,
+                                                    const emel_paged_attn_options* options);
+
+/* Rows of 4-bit weights laid out for emel_cuda_mul_mat_q4: the caller's device
+ * buffer `data` of `bytes`, filled once by emel_cuda_q4_pack. */
+typedef struct emel_q4_weights {
+    void* data;
+    uint64_t bytes;
+    uint64_t k;     /* weights of a row */
+    uint64_t rows;
+    uint32_t dtype; /* EMEL_DTYPE_Q4_0, Q4_1 or Q4_K: the format packed from */
+    uint32_t reserved; /* 0 */
+} emel_q4_weights;
+/* Bytes of the packed form of `rows` rows of `k` weights (k a multiple of 32,
+ * or 256 for Q4_K): the source's size, rounded up to tiles of 16 rows and
+ * 64 columns (Q4_K: and 3 % more).  INVALID_ARGUMENT for anything else. */
+EMEL_CUDA_API emel_cuda_status emel_cuda_q4_packed_bytes(uint32_t dtype, uint64_t k, uint64_t rows, uint64_t* bytes);
+/* Lays out src (packed rows as in emel_cuda_mul_mat_argmax_q4_0 /
+ * emel_gguf_tensor_view: [k, rows], two-dimensional) into `data` and fills
+ * *out.  Statuses: INVALID_VIEW, SHAPE_MISMATCH (more than two dimensions),
+ * CAPACITY (bytes too small), INVALID_ARGUMENT (null or not 16-byte aligned
+ * data, overlap with src, null out or context). */
+EMEL_CUDA_API emel_cuda_status emel_cuda_q4_pack(emel_cuda_context* ctx, void* stream, const emel_tensor_view* src,
+                                                 void* data, uint64_t bytes, emel_q4_weights* out);
+/* dst[r, i] = sum over c of w[r, c] * rhs[c, i]: rhs [k, n] F32 or F16, dst
+ * [rows, n] F32 or F16, unit rows.  Weights count with their exact values
+ * (d (q - 8), d q + m, d s q - e t), products are exact and sums binary32,
+ * rounded once to dst's type.  A matrix-vector product for single tokens and
+ * small batches: every further 8 columns of rhs read the weights once more.
+ * Weights' scales must be finite.
+ * Statuses: INVALID_VIEW (views or weights), INVALID_LAYOUT, SHAPE_MISMATCH,
+ * INVALID_ARGUMENT (null context, dst overlapping rhs or the weights). */
+EMEL_CUDA_API emel_cuda_status emel_cuda_mul_mat_q4(emel_cuda_context* ctx, void* stream,
+                                                    const emel_q4_weights* weights, const emel_tensor_view* rhs,
+                                                    const emel_tensor_view* dst);
+
+/* Logits before a token is chosen.  src and dst are [vocab, rows], F32 or F16
+ * (both the same), unit rows; dst may be src itself.  For token i with value
+ * v, in binary32 and rounded once to dst's type:
+ *   history (I32 [capacity, rows]), history_lengths (I32 [rows]) and penalties
+ *     (F32 [3, rows] or [3, 1]: repetition r, frequency f, presence p), all
+ *     three or none: c = how often i stands in the row's first
+ *     history_lengths ids; c > 0: v = v > 0 ? v / r : v * r, v = v - c f - p.
+ *     Ids outside the vocabulary are passed over, a length counts at most
+ *     the capacity;
+ *   bias (F32 [vocab, rows] or [vocab, 1], unit rows; nullable): v = v + bias;
+ *   allowed (I32 [ceil(vocab / 32), rows] or [.., 1], unit rows; nullable):
+ *     v = -inf where bit i % 32 of word i / 32 is 0, whatever v was.
+ * Statuses: INVALID_VIEW (also a partial history), INVALID_LAYOUT,
+ * SHAPE_MISMATCH, INVALID_ARGUMENT (null context, dst overlapping an input
+ * otherwise than as src itself, or more than 2^31 - 1 pieces of 8192 logits). */
+EMEL_CUDA_API emel_cuda_status emel_cuda_logits_adjust(emel_cuda_context* ctx, void* stream,
+                                                       const emel_tensor_view* src, const emel_tensor_view* history,
+                                                       const emel_tensor_view* history_lengths,
+                                                       const emel_tensor_view* penalties,
+                                                       const emel_tensor_view* bias, const emel_tensor_view* allowed,
+                                                       const emel_tensor_view* dst);
+
 /* ---- peer exchange over NVLink (multi-GPU partials) -------------------- */
 /* One process per GPU shards a tensor; each rank's small partial (the f64
  * sum and the emel_cuda_argmax_partial of its shard) must reach every rank.
