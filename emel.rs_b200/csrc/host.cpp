@@ -23,6 +23,7 @@ struct emel_cuda_context {
     int sm_count;
     void* workspace;
     uint64_t workspace_bytes;
+    uint64_t paged_offset;  // the paged attention's pieces and tickets in the workspace
     void* tables;  // binary16 domain tables, built at creation
     uint64_t launches;
     uint64_t fa_prepared_tokens;  // FlashAttnWorkspace::prepared_tokens (flash_attn.rs:117-118)
@@ -443,7 +444,8 @@ emel_cuda_status emel_cuda_context_create(int device, emel_cuda_context** out) {
     cudaError_t err = cudaSetDevice(device);
     if (err == cudaSuccess) err = cudaDeviceGetAttribute(&ctx->sm_count, cudaDevAttrMultiProcessorCount, device);
     if (err == cudaSuccess) {
-        ctx->workspace_bytes = emel::reduction_workspace_bytes(ctx->sm_count);
+        ctx->paged_offset = (emel::reduction_workspace_bytes(ctx->sm_count) + 255) / 256 * 256;
+        ctx->workspace_bytes = ctx->paged_offset + emel::paged_workspace_bytes(ctx->sm_count);
         err = cudaMalloc(&ctx->workspace, ctx->workspace_bytes);
     }
     if (err == cudaSuccess) err = cudaMemset(ctx->workspace, 0, ctx->workspace_bytes);
@@ -1843,6 +1845,15 @@ emel_cuda_status emel_cuda_paged_attn(emel_cuda_context* ctx, void* stream, cons
     p.scale = scale;
     p.q_f32 = query->dtype == EMEL_DTYPE_F32;
     p.cache_bf16 = key_cache->dtype == EMEL_DTYPE_BF16;
+    auto rows16 = [](const emel_tensor_view* v, const Checked& c) {
+        bool ok = aligned16(v->data);
+        for (int i = 1; i < 4; ++i) ok = ok && (v->ne[i] == 1 || c.nb[i] % 16 == 0);
+        return ok;
+    };
+    p.vec = d % 8 == 0 && rows16(key_cache, ck) && rows16(value_cache, cv);
+    char* pieces = static_cast<char*>(ctx->workspace) + ctx->paged_offset;
+    p.pieces = reinterpret_cast<float*>(pieces);
+    p.tickets = reinterpret_cast<uint32_t*>(pieces + emel::paged_piece_bytes(ctx->sm_count));
     p.reject = reject_word(ctx);
     p.reject_code = EMEL_CUDA_INDEX_OUT_OF_BOUNDS;
     cudaError_t err = select_device(ctx);

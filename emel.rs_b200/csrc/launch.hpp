@@ -246,12 +246,21 @@ struct PagedAttnPlan {
     int64_t len_st;
     uint64_t d, heads, batch, rep, page_size, pages;
     uint64_t window;        // 0: every cached token is seen
+    uint64_t min_run;       // tiles of a CTA at least (set by the launcher)
     float scale;
     bool q_f32, cache_bf16;
+    bool vec;               // d % 8 == 0 and every cache row 16-byte aligned
+    float* pieces;          // workspace: two pieces per CTA
+    uint32_t* tickets;      // workspace: one per CTA, zero between calls
     uint32_t* reject;
     uint32_t reject_code;
 };
 
+// Workspace of the attention: pieces of sequences cut between CTAs, and their
+// tickets.
+uint64_t paged_piece_bytes(int sm_count);
+uint64_t paged_tickets(int sm_count);
+inline uint64_t paged_workspace_bytes(int sm_count) { return paged_piece_bytes(sm_count) + paged_tickets(sm_count) * 4; }
 cudaError_t launch_paged_attn(const LaunchEnv& env, const PagedAttnPlan& plan);
 
 // Matrix-vector products with 4-bit weights (q4.cu); code: the rows' dtype.

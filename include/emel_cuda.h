@@ -785,7 +785,8 @@ EMEL_CUDA_API emel_cuda_status emel_cuda_paged_kv_append(emel_cuda_context* ctx,
  * n = lengths[b] and t over [window ? max(0, n - window) : 0, n):
  *     s_t = scale * q . k_t,   dst = sum exp(s_t - max s) v_t / sum exp(s_t - max s)
  * A sequence without tokens (n <= 0) gives zeros, and so does one whose every
- * score is -inf.  Whatever lies in the cache beyond the n tokens (or before
+ * score is -inf; a NaN or +inf score, or a value that is not finite, gives
+ * what is not finite.  Whatever lies in the cache beyond the n tokens (or before
  * the window) has no effect, NaN and infinities included.  Scores, weights'
  * sums and products are binary32; 16-bit queries round the weights to the
  * cache's type before they meet the values.  A length beyond the table
