@@ -1910,7 +1910,7 @@ emel_cuda_status emel_cuda_mul_mat_q4(emel_cuda_context* ctx, void* stream, cons
         return EMEL_CUDA_INVALID_VIEW;
     if (!unit_rows(rhs, cr) || !unit_rows(dst, cd)) return EMEL_CUDA_INVALID_LAYOUT;
     const uint64_t n = rhs->ne[1];
-    if (rhs->ne[0] != weights->k || rhs->ne[2] != 1 || rhs->ne[3] != 1 || dst->ne[0] != weights->rows ||
+    if (weights->k > emel::kQ4MaxK || rhs->ne[0] != weights->k || rhs->ne[2] != 1 || rhs->ne[3] != 1 || dst->ne[0] != weights->rows ||
         dst->ne[1] != n || dst->ne[2] != 1 || dst->ne[3] != 1)
         return EMEL_CUDA_SHAPE_MISMATCH;
     if (ctx == nullptr || views_overlap(dst, cd, rhs, cr) ||

@@ -264,6 +264,7 @@ inline uint64_t paged_workspace_bytes(int sm_count) { return paged_piece_bytes(s
 cudaError_t launch_paged_attn(const LaunchEnv& env, const PagedAttnPlan& plan);
 
 // Matrix-vector products with 4-bit weights (q4.cu); code: the rows' dtype.
+constexpr uint64_t kQ4MaxK = 131072;  // a column of x, cut over a cluster, has to fit in shared memory
 struct Q4PackPlan {
     const uint8_t* src;     // rows of k / 32 or k / 256 blocks
     uint8_t* dst;           // packed layout, 16-byte aligned

@@ -836,8 +836,10 @@ EMEL_CUDA_API emel_cuda_status emel_cuda_q4_pack(emel_cuda_context* ctx, void* s
  * (d (q - 8), d q + m, d s q - e t), products are exact and sums binary32,
  * rounded once to dst's type.  A matrix-vector product for single tokens and
  * small batches: every further 8 columns of rhs read the weights once more.
- * Weights' scales must be finite.
- * Statuses: INVALID_VIEW (views or weights), INVALID_LAYOUT, SHAPE_MISMATCH,
+ * Weights' scales must be finite.  An F32 activation counts with 22 bits or
+ * more of its value, down to 2^-40 of its column's largest finite one.
+ * Statuses: INVALID_VIEW (views or weights), INVALID_LAYOUT, SHAPE_MISMATCH
+ * (k > 131072 among them),
  * INVALID_ARGUMENT (null context, dst overlapping rhs or the weights). */
 EMEL_CUDA_API emel_cuda_status emel_cuda_mul_mat_q4(emel_cuda_context* ctx, void* stream,
                                                     const emel_q4_weights* weights, const emel_tensor_view* rhs,
