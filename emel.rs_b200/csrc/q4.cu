@@ -121,17 +121,29 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackPlan p) {
 //
 // Reading the weights once is what bounds it (4.5 bits each); the work per
 // weight has to stay under what an SM can issue while it waits for them: about
-// three instructions a weight at full bandwidth.  So the quants become binary16
-// integers q - 8 two at a time (a mask that leaves 1024 + q or 1024 + 16 q, one
-// subtraction or multiply-add: exact), and m16n8k16 products multiply 16 rows
-// with up to 8 columns of x at once, one instruction for 8 weights a lane.  The
-// scales meet the products of a group, in binary32.
+// three instructions a weight at full bandwidth, shared by all pipes.  So
+// tensor products multiply 16 rows with 8 columns at once, and the quants reach
+// them with as little work as the number of tokens allows.
 //
-// Columns of x.  binary16: one for each token, as it is.  binary32: two for
-// each token, x 2^e = hi + lo with both rounded to binary16 and e chosen per
-// token (and CTA) so that the largest |x| lies in [2^14, 2^15): 22 bits and
-// more, down to 2^-40 of the largest.  The tensor pipe is idle otherwise, so
-// the second column costs no time.
+// One or two tokens (q4_digits_kernel, m16n8k32 on 8-bit integers): a mask
+// leaves four quants of a word, a shift and a mask the other four, three
+// instructions for 8 weights.  A token is x 2^e rounded to an integer of 31
+// bits (e per token and CTA: the largest finite |x| in [2^29, 2^30)), and its four
+// balanced digits to the base 256 are four columns.  A group's integer sum is exact; it
+// comes out of the product on top of the bits of 1.5 2^23, so that one
+// subtraction, of that plus 8 times the digits' sum, makes sum((q - 8) digit) a
+// binary32 number.
+//
+// More tokens (q4_halves_kernel, m16n8k16 on binary16): a mask leaves the bits
+// of 1024 + q or, four bits higher up, of 1024 + 16 q, one subtraction or
+// multiply-add makes q - 8 of them, exactly; nine instructions for 8 weights.
+// (The masked bits alone, as the subnormals q 2^-24, would take five, but the
+// tensor pipe adds products of subnormals with seven bits less.)  A binary16
+// token is one column as it is; a binary32 token is two, x 2^e = hi + lo, both
+// rounded to binary16, the largest finite |x| in [2^14, 2^15): 22 bits and more, down to
+// 2^-40 of the largest.
+//
+// The scales meet the products of a group, in binary32.
 //
 // A persistent CTA of 16 warps keeps its columns of x in shared memory and
 // walks tiles of 16 rows.  WK warps share a tile (each a part of its 256-column
@@ -143,6 +155,7 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackPlan p) {
 constexpr int kQ4Warps = 16;
 constexpr int kQ4MulThreads = kQ4Warps * 32;
 constexpr int kQ4Tokens = 8;  // columns of one launch
+constexpr int kQ4DigitTokens = 2;
 
 struct Q4Shape {
     uint32_t wk, wr;       // warps of a tile, tiles in work: wk * wr = kQ4Warps
@@ -154,87 +167,112 @@ struct Q4Shape {
     bool early, x_vec;
 };
 
-__device__ __forceinline__ uint4 ld_weights(const uint4* p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
+// Loads into v where `in`; v keeps its value otherwise.
+__device__ __forceinline__ void load_if(uint4& v, const uint4* p, bool in) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+        "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+        : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+        : "l"(p), "r"((uint32_t)in));
+}
+__device__ __forceinline__ void load_if(uint2& v, const uint2* p, bool in) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\t"
+        "@p ld.global.nc.v2.u32 {%0,%1}, [%2];\n\t}"
+        : "+r"(v.x), "+r"(v.y)
+        : "l"(p), "r"((uint32_t)in));
 }
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+// d = a b + 0
+__device__ __forceinline__ void mma_half(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// d += a b
+__device__ __forceinline__ void mma_half_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// d = a b + c in every element, integers
+__device__ __forceinline__ void mma_digits(uint32_t (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                           uint32_t b0, uint32_t b1, uint32_t c) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c));
 }
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 bits_h2(uint32_t u) { return *reinterpret_cast<const __half2*>(&u); }
 
-// (w & mask) | 0x64006400 in one instruction.
+// (w & MASK) | base in one instruction
 template <uint32_t MASK>
-__device__ __forceinline__ uint32_t biased(uint32_t w) {
+__device__ __forceinline__ uint32_t mask_or(uint32_t w, uint32_t base) {
     uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(MASK), "r"(0x64006400u));
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "n"(MASK), "r"(base));
     return r;
 }
 
-// The eight quants of a word as q - 8: operand registers 0..3.
-__device__ __forceinline__ void quants(uint32_t w, uint32_t (&a)[4]) {
+// The eight quants of a word as binary16 q - 8: operand registers 0..3.
+__device__ __forceinline__ void half_quants(uint32_t w, uint32_t (&a)[4]) {
     const __half2 b1032 = __half2half2(__ushort_as_half(0x6408));  // 1024 + 8
     const __half2 b72 = __half2half2(__ushort_as_half(0xd480)), b16 = __half2half2(__ushort_as_half(0x2c00));  // -72, 1/16
-    const uint32_t v = w >> 8;
-    a[0] = h2_bits(__hsub2(bits_h2(biased<0x000f000fu>(w)), b1032));
-    a[1] = h2_bits(__hfma2(bits_h2(biased<0x00f000f0u>(w)), b16, b72));
-    a[2] = h2_bits(__hsub2(bits_h2(biased<0x000f000fu>(v)), b1032));
-    a[3] = h2_bits(__hfma2(bits_h2(biased<0x00f000f0u>(v)), b16, b72));
+    const uint32_t v = w >> 8, base = 0x64006400u;
+    a[0] = h2_bits(__hsub2(bits_h2(mask_or<0x000f000fu>(w, base)), b1032));
+    a[1] = h2_bits(__hfma2(bits_h2(mask_or<0x00f000f0u>(w, base)), b16, b72));
+    a[2] = h2_bits(__hsub2(bits_h2(mask_or<0x000f000fu>(v, base)), b1032));
+    a[3] = h2_bits(__hfma2(bits_h2(mask_or<0x00f000f0u>(v, base)), b16, b72));
 }
 
 // Scales of one 256-column block as a lane holds them: of its 64-column block
 // t, slots (row g, group 0), (g, 1), (g + 8, 0), (g + 8, 1).
 template <int CODE>
 struct Q4Scales {
-    uint32_t r[CODE == kDtypeQ4_0 ? 2 : 4];
-    __device__ __forceinline__ void load(const uint8_t* rec, uint32_t lane) {
-        if constexpr (CODE == kDtypeQ4_0) {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(rec) + lane);
-            r[0] = v.x;
-            r[1] = v.y;
-        } else if constexpr (CODE == kDtypeQ4_1) {
-            const uint4 v = ld_weights(reinterpret_cast<const uint4*>(rec) + lane);
-            r[0] = v.x, r[1] = v.y, r[2] = v.z, r[3] = v.w;
+    uint4 r;  // Q4_0: x, y; Q4_K: x, y and the (d, e) of its two rows
+    __device__ __forceinline__ void load(const uint8_t* rec, uint32_t lane, bool in) {
+        if constexpr (CODE == kDtypeQ4_1) {
+            load_if(r, reinterpret_cast<const uint4*>(rec) + lane, in);
         } else {
-            const uint2 v = __ldg(reinterpret_cast<const uint2*>(rec) + lane);
-            const uint2 de = __ldg(reinterpret_cast<const uint2*>(rec + 256) + (lane >> 2));
-            r[0] = v.x, r[1] = v.y, r[2] = de.x, r[3] = de.y;
+            uint2 v = make_uint2(r.x, r.y);
+            load_if(v, reinterpret_cast<const uint2*>(rec) + lane, in);
+            r.x = v.x, r.y = v.y;
+            if constexpr (CODE == kDtypeQ4_K) {
+                uint2 de = make_uint2(r.z, r.w);
+                load_if(de, reinterpret_cast<const uint2*>(rec + 256) + (lane >> 2), in);
+                r.z = de.x, r.w = de.y;
+            }
         }
     }
-    // a[row half][group], c likewise, of 64-column block j
+    // a[row half][group], c likewise (Q4_0: not used), of 64-column block j
     __device__ __forceinline__ void of(uint32_t lane, int j, float (&a)[2][2], float (&c)[2][2]) const {
         const uint32_t from = (lane & 28u) | (uint32_t)j;
         if constexpr (CODE == kDtypeQ4_0) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float2 f = __half22float2(bits_h2(__shfl_sync(0xffffffffu, r[h], from)));
+                const float2 f = __half22float2(bits_h2(__shfl_sync(0xffffffffu, h ? r.y : r.x, from)));
                 a[h][0] = f.x;
                 a[h][1] = f.y;
             }
         } else if constexpr (CODE == kDtypeQ4_1) {
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-                const float2 f = __half22float2(bits_h2(__shfl_sync(0xffffffffu, r[s], from)));
+                const float2 f = __half22float2(bits_h2(__shfl_sync(0xffffffffu, w[s], from)));
                 a[s >> 1][s & 1] = f.x;
                 c[s >> 1][s & 1] = __fmaf_rn(8.0f, f.x, f.y);
             }
         } else {
+            // a byte under the exponent of 2^23 is 2^23 + byte
+            const auto value = [](uint32_t b, uint32_t at) { return bitsf(__byte_perm(b, 0x4b000000u, 0x7440u + at)) - 8388608.0f; };
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float2 de = __half22float2(bits_h2(r[2 + h]));
-                const uint32_t b = __shfl_sync(0xffffffffu, r[h], from);
+                const float2 de = __half22float2(bits_h2(h ? r.w : r.z));
+                const uint32_t b = __shfl_sync(0xffffffffu, h ? r.y : r.x, from);
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    a[h][s] = de.x * (float)((b >> (16 * s)) & 255u);
-                    c[h][s] = __fmaf_rn(8.0f, a[h][s], -de.y * (float)((b >> (16 * s + 8)) & 255u));
+                    a[h][s] = de.x * value(b, 2 * s);
+                    c[h][s] = __fmaf_rn(8.0f, a[h][s], -de.y * value(b, 2 * s + 1));
                 }
             }
         }
@@ -247,179 +285,372 @@ struct Q4Block {
     Q4Scales<CODE> s;
 };
 
+// Where a CTA and a warp stand: their parts of k and of the tiles.
+struct Q4Place {
+    uint64_t tiles, k64, k256;
+    uint32_t lane, warp, wk, wr, rank, group;
+    uint32_t first, here;  // the CTA's 256-column blocks
+    uint32_t kb0, kb1;     // the warp's, from `first` on
+    __device__ __forceinline__ Q4Place(const Q4MatvecPlan& p, const Q4Shape& shape) {
+        lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+        rank = shape.splits > 1 ? blockIdx.x % shape.splits : 0;
+        group = shape.splits > 1 ? blockIdx.x / shape.splits : blockIdx.x;
+        tiles = (p.rows + 15) / 16, k64 = (p.k + 63) / 64, k256 = (p.k + 255) / 256;
+        first = rank * shape.blocks;
+        here = first >= k256 ? 0u : (uint32_t)(k256 - first < shape.blocks ? k256 - first : shape.blocks);
+        wk = warp % shape.wk, wr = warp / shape.wk;
+        kb0 = wk * here / shape.wk, kb1 = (wk + 1) * here / shape.wk;
+    }
+};
+
+// A warp's blocks in order: tiles group * wr + ..., of each kb0 .. kb1.  Quads
+// that do not exist (the last block of a row may hold less than four) keep
+// old bits: the columns of x under them are zeros, and so are their scales.
+template <int CODE>
+struct Q4Stream {
+    const uint4* q;
+    const uint8_t* s;
+    uint64_t q_step, s_step;  // from the end of a tile's part to the next tile's
+    uint32_t kb, kb0, kb1, left, lane, short_kb, short_n, quads;
+    __device__ __forceinline__ Q4Stream(const Q4MatvecPlan& p, const Q4Shape& shape, const Q4Place& w) {
+        const uint64_t tile = (uint64_t)w.group * shape.wr + w.wr, step = (uint64_t)shape.groups * shape.wr;
+        lane = w.lane;
+        kb = kb0 = w.kb0;
+        kb1 = w.kb1;
+        left = kb0 == kb1 || tile >= w.tiles ? 0u : (uint32_t)((w.tiles - 1 - tile) / step) + 1;
+        q = reinterpret_cast<const uint4*>(p.weights) + (tile * w.k64 + (uint64_t)(w.first + kb0) * 4) * 32 + lane;
+        s = p.weights + w.tiles * w.k64 * 512 + (tile * w.k256 + w.first + kb0) * q4_scale_bytes(CODE);
+        q_step = (step * w.k64 - (uint64_t)(kb1 - kb0) * 4) * 32;
+        s_step = (step * w.k256 - (kb1 - kb0)) * q4_scale_bytes(CODE);
+        short_kb = w.first + w.here == w.k256 && (w.k64 & 3u) ? w.here - 1 : 0xffffffffu;
+        short_n = (uint32_t)w.k64 & 3u;
+        count();
+    }
+    __device__ __forceinline__ void count() { quads = left == 0 ? 0u : kb == short_kb ? short_n : 4u; }
+    __device__ __forceinline__ void fetch_quads(Q4Block<CODE>& b, int j) { load_if(b.q[j], q + j * 32, (uint32_t)j < quads); }
+    __device__ __forceinline__ void fetch_scales(Q4Block<CODE>& b) { b.s.load(s, lane, quads != 0); }
+    __device__ __forceinline__ void next() {
+        q += 128;
+        s += q4_scale_bytes(CODE);
+        if (++kb == kb1) {
+            kb = kb0;
+            q += q_step;
+            s += s_step;
+            left -= left != 0;
+        }
+        count();
+    }
+    __device__ __forceinline__ void fill(Q4Block<CODE> (&b)[2]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            fetch_scales(b[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) fetch_quads(b[i], j);
+            next();
+        }
+    }
+};
+
+// Pieces of 8 values of x, shared out over the CTA; a warp stays in one token.
+struct Q4Piece {
+    uint32_t token, at;
+    __device__ __forceinline__ void next(uint32_t pieces) {
+        at += kQ4MulThreads;
+        while (at >= pieces) {
+            at -= pieces;
+            ++token;
+        }
+    }
+};
+
+// The 8 values of a piece as they lie in memory: 16 bytes of binary16, or 32 of
+// binary32; zeros beyond k (a multiple of 32: no piece is cut).
+template <bool F32>
+__device__ __forceinline__ void load_piece(const Q4MatvecPlan& p, bool vec, uint64_t k, uint32_t token, bool in, uint4 (&v)[F32 ? 2 : 1]) {
+    const char* src = p.x + token * p.x_st + k * (F32 ? 4 : 2);
+#pragma unroll
+    for (int h = 0; h < (F32 ? 2 : 1); ++h) v[h] = make_uint4(0, 0, 0, 0);
+    if (!in || k >= p.k) return;
+    if (vec) {
+#pragma unroll
+        for (int h = 0; h < (F32 ? 2 : 1); ++h) v[h] = *reinterpret_cast<const uint4*>(src + 16 * h);
+        return;
+    }
+    uint32_t w[8];
+#pragma unroll
+    for (int e = 0; e < (F32 ? 8 : 4); ++e) {
+        if constexpr (F32) w[e] = reinterpret_cast<const uint32_t*>(src)[e];
+        else w[e] = reinterpret_cast<const uint16_t*>(src)[2 * e] | (uint32_t)reinterpret_cast<const uint16_t*>(src)[2 * e + 1] << 16;
+    }
+    v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (F32) v[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+// The largest finite magnitude (bits) among eight binary32 values.
+__device__ __forceinline__ uint32_t largest_of(const uint32_t (&w)[8]) {
+    uint32_t big = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t b = w[e] & 0x7fffffffu;
+        big = b < 0x7f800000u && b > big ? b : big;
+    }
+    return big;
+}
+
+// The power of two that brings `largest` (bits) into [2^to, 2^(to + 1)), as far
+// as it is a normal number.
+__device__ __forceinline__ float scale_to(uint32_t largest, int to) {
+    const int e = 127 + to + 127 - (int)(largest >> 23);
+    return largest == 0 ? 1.0f : bitsf((uint32_t)(e > 254 ? 254 : e) << 23);
+}
+
+// The sums of a round: every warp's [16 rows][COLS] lie in shared memory, 8
+// floats apart beyond their size; the output (tile, row, token) is the sum over
+// its WK warps and PARTS columns, part i weighted by `weight`^i.  Four lanes, 8
+// apart, share an output: lane quarter s takes warps s, s + 4, ..., so the 32
+// lanes read 32 banks.
+constexpr uint32_t kQ4RedPad = 8;
+template <int PARTS, int COLS>
+__device__ __forceinline__ void q4_join(const Q4MatvecPlan& p, const Q4Shape& shape, const Q4Place& w, uint32_t round,
+                                        const float* sums, float* part, const float* up, float weight) {
+    constexpr uint32_t kWarp = 16 * COLS + kQ4RedPad;
+    const uint32_t n = (uint32_t)p.n, outs = shape.wr * 16 * n, over_n = (65535 + n) / n;
+    const uint64_t row0 = ((uint64_t)round * shape.groups + w.group) * shape.wr * 16;
+    auto store = [&](uint32_t row, uint32_t token, float y) {
+        const uint64_t r = row0 + row;
+        if (r >= p.rows) return;
+        char* at = p.dst + token * p.dst_st;
+        if (p.dst_f16) reinterpret_cast<__half*>(at)[r] = __float2half_rn(y);
+        else reinterpret_cast<float*>(at)[r] = y;
+    };
+    const uint32_t quarter = w.lane >> 3;
+    for (uint32_t base = w.warp * 8; base < outs; base += kQ4Warps * 8) {
+        const uint32_t o = base + (w.lane & 7u);  // outs is a multiple of 8
+        const uint32_t row = (o * over_n) >> 16, token = o - row * n;  // o / n, exact for o <= 2048, n <= 8
+        float y[PARTS] = {};
+        const float* at = sums + ((row >> 4) * shape.wk + quarter) * kWarp + (row & 15u) * COLS + token;
+#pragma unroll 4
+        for (uint32_t v = quarter; v < shape.wk; v += 4, at += 4 * kWarp)
+#pragma unroll
+            for (int i = 0; i < PARTS; ++i) y[i] += at[i * n];
+        float all = y[PARTS - 1];
+#pragma unroll
+        for (int i = PARTS - 2; i >= 0; --i) all = __fmaf_rn(all, weight, y[i]);
+        all += __shfl_xor_sync(0xffffffffu, all, 8);
+        all += __shfl_xor_sync(0xffffffffu, all, 16);
+        if (quarter == 0) {
+            all *= up[token];
+            if (shape.splits > 1) part[(round & 1u) * outs + o] = all;
+            else store(row, token, all);
+        }
+    }
+    if (shape.splits > 1) {
+        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        cluster.sync();
+        for (uint32_t o = threadIdx.x * shape.splits + w.rank; o < outs; o += kQ4MulThreads * shape.splits) {
+            const uint32_t row = (o * over_n) >> 16, token = o - row * n;
+            float y = 0.0f;
+            for (uint32_t r = 0; r < shape.splits; ++r) y += cluster.map_shared_rank(part, r)[(round & 1u) * outs + o];
+            store(row, token, y);
+        }
+    }
+}
+
+// Walks the rounds: `work(block, kb)` adds one block to the warp's `total`.
+template <int CODE, int PARTS, int NT, typename Work>
+__device__ __forceinline__ void q4_rounds(const Q4MatvecPlan& p, const Q4Shape& shape, const Q4Place& w, Q4Block<CODE> (&blk)[2],
+                                          float (&total)[NT][4], float* red, float* part, const float* up, float weight,
+                                          Work&& work) {
+    constexpr int kCols = 8 * NT;
+    const uint32_t g = w.lane >> 2, t = w.lane & 3u;
+    uint32_t odd = 0;  // which of the two blocks comes next
+    for (uint32_t round = 0; round < shape.rounds; ++round) {
+#pragma unroll
+        for (int m = 0; m < NT; ++m) total[m][0] = total[m][1] = total[m][2] = total[m][3] = 0.0f;
+        uint32_t kb = w.kb0;
+        if (((uint64_t)round * shape.groups + w.group) * shape.wr + w.wr < w.tiles) {
+            if (odd && kb < w.kb1) {
+                work(blk[1], kb++);
+                odd = 0;
+            }
+            for (; kb + 2 <= w.kb1; kb += 2) {
+                work(blk[0], kb);
+                work(blk[1], kb + 1);
+            }
+            if (kb < w.kb1) {
+                work(blk[0], kb);
+                odd = 1;
+            }
+        }
+        float* sums = red + (round & 1u) * kQ4Warps * (16 * kCols + kQ4RedPad);
+        float* mine = sums + w.warp * (16 * kCols + kQ4RedPad);
+#pragma unroll
+        for (int m = 0; m < NT; ++m) {
+            *reinterpret_cast<float2*>(mine + g * kCols + 8 * m + 2 * t) = make_float2(total[m][0], total[m][1]);
+            *reinterpret_cast<float2*>(mine + (g + 8) * kCols + 8 * m + 2 * t) = make_float2(total[m][2], total[m][3]);
+        }
+        __syncthreads();
+        q4_join<PARTS, kCols>(p, shape, w, round, sums, part, up, weight);
+    }
+    if (shape.splits > 1) cooperative_groups::this_cluster().sync();  // the others may still read this CTA's part
+}
+
+// Shared memory of both kernels: the warps' sums, the cluster's, the tokens'
+// scales, tables of the groups and the columns of x.
+template <int NT>
+struct Q4Shared {
+    float* red;      // [2][warp][16][8 NT], padded
+    float* part;     // [2][wr * 16 * n], splits > 1
+    float* up;       // [kQ4Tokens]: 2^-e
+    uint32_t* top;   // [kQ4Tokens]: bits of the largest finite |x|
+    float* table;    // per group
+    unsigned char* xs;
+    __device__ __forceinline__ Q4Shared(unsigned char* smem, const Q4Shape& shape, uint32_t n, uint32_t table_floats) {
+        red = reinterpret_cast<float*>(smem);
+        part = red + 2 * kQ4Warps * (16 * 8 * NT + kQ4RedPad);
+        up = part + (shape.splits > 1 ? 2 * shape.wr * 16 * n : 0);
+        top = reinterpret_cast<uint32_t*>(up + kQ4Tokens);
+        table = reinterpret_cast<float*>(top + kQ4Tokens);
+        xs = reinterpret_cast<unsigned char*>(table + shape.blocks * 8 * table_floats);
+    }
+};
+
+constexpr int kQ4Batch = 4, kQ4DigitBatch = 2;  // pieces of x that a thread has in flight
+
+// PARTS columns a token (1: binary16 x, 2: binary32 x), NT * 8 columns.
 template <int CODE, int PARTS, int NT>
-__global__ void __launch_bounds__(kQ4MulThreads, 1) q4_mul_kernel(const Q4MatvecPlan p, const Q4Shape shape) {
+__global__ void __launch_bounds__(kQ4MulThreads, 1) q4_halves_kernel(const Q4MatvecPlan p, const Q4Shape shape) {
     constexpr int kCols = 8 * NT;
     constexpr bool kSums = CODE != kDtypeQ4_0;
     extern __shared__ __align__(16) unsigned char smem[];
     const uint32_t n = (uint32_t)p.n, cols = n * PARTS;
-    float* red = reinterpret_cast<float*>(smem);                          // [2][warp][16][kCols]
-    float* part = red + 2 * kQ4Warps * 16 * kCols;                        // [2][wr * 16 * n], splits > 1
-    float* up = part + (shape.splits > 1 ? 2 * shape.wr * 16 * n : 0);    // [8]
-    uint32_t* top = reinterpret_cast<uint32_t*>(up + kQ4Tokens);          // [8]
-    float* xsum = reinterpret_cast<float*>(top + kQ4Tokens);              // [group][kCols]
-    unsigned char* xs = reinterpret_cast<unsigned char*>(xsum + (kSums ? shape.blocks * 8 * kCols : 0));
-
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3u;
-    const uint32_t rank = shape.splits > 1 ? blockIdx.x % shape.splits : 0;
-    const uint32_t group = shape.splits > 1 ? blockIdx.x / shape.splits : blockIdx.x;
-    const uint64_t tiles = (p.rows + 15) / 16, k64 = (p.k + 63) / 64, k256 = (p.k + 255) / 256;
-    const uint4* quads = reinterpret_cast<const uint4*>(p.weights);
-    const uint8_t* scales = p.weights + tiles * k64 * 512;
-    const uint32_t first = rank * shape.blocks;  // of this CTA's blocks
-    const uint32_t here = first >= k256 ? 0u : (uint32_t)(k256 - first < shape.blocks ? k256 - first : shape.blocks);
-    const uint32_t wk = warp % shape.wk, wr = warp / shape.wk;
-    const uint32_t kb0 = wk * here / shape.wk, kb1 = (wk + 1) * here / shape.wk;
-
-    // this warp's sequence of (tile, block): tiles group * wr + ..., blocks kb0 .. kb1
-    struct At {
-        uint64_t tile;
-        uint32_t kb, round;
-    };
-    At ahead{(uint64_t)group * shape.wr + wr, kb0, 0};
-    auto fetch_quads = [&](Q4Block<CODE>& b, const At& x, int j) {
-        const uint64_t block = (uint64_t)(first + x.kb) * 4 + j;
-        b.q[j] = x.round < shape.rounds && x.tile < tiles && block < k64 ? ld_weights(quads + (x.tile * k64 + block) * 32 + lane)
-                                                                         : make_uint4(0, 0, 0, 0);
-    };
-    auto fetch_scales = [&](Q4Block<CODE>& b, const At& x) {
-        if (x.round < shape.rounds && x.tile < tiles)
-            b.s.load(scales + (x.tile * k256 + first + x.kb) * q4_scale_bytes(CODE), lane);
-    };
-    auto next = [&](At& x) {
-        if (++x.kb == kb1) {
-            x.kb = kb0;
-            x.tile += (uint64_t)shape.groups * shape.wr;
-            ++x.round;
-        }
-    };
+    const Q4Shared<NT> sh(smem, shape, n, kSums ? kCols : 0);
+    const Q4Place w(p, shape);
+    Q4Stream<CODE> ahead(p, shape, w);
     Q4Block<CODE> blk[2] = {};
-    auto fill = [&]() {
-        if (kb0 == kb1) return;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            fetch_scales(blk[s], ahead);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) fetch_quads(blk[s], ahead, j);
-            next(ahead);
-        }
-    };
-    if (shape.early) fill();  // the previous kernel of the stream does not write the weights
+    if (shape.early) ahead.fill(blk);  // the previous kernel of the stream does not write the weights
     pdl_enter();
-    if (!shape.early) fill();
+    if (!shape.early) ahead.fill(blk);
 
     // ---- the columns of x
-    const uint32_t pieces = here * 32;  // 8 values each; a multiple of 32: a warp stays in one token
-    auto load8 = [&](uint32_t i, float (&v)[8]) {
-        const uint32_t token = i / pieces;
-        const uint64_t k = (uint64_t)first * 256 + (uint64_t)(i % pieces) * 8;
-        const char* row = p.x + token * p.x_st;
-        if constexpr (PARTS == 2) {
-            const float* src = reinterpret_cast<const float*>(row) + k;
-            if (shape.x_vec && k + 8 <= p.k) {
-                const float4 lo = *reinterpret_cast<const float4*>(src), hi = *reinterpret_cast<const float4*>(src + 4);
-                v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w, v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = k + e < p.k ? src[e] : 0.0f;
-            }
-        } else {
-            const __half* src = reinterpret_cast<const __half*>(row) + k;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = k + e < p.k ? __half2float(src[e]) : 0.0f;
-        }
-    };
-    if (here == 0 && threadIdx.x < kQ4Tokens) up[threadIdx.x] = 1.0f;  // a part of k beyond the matrix
-    if constexpr (PARTS == 2) {
-        if (threadIdx.x < kQ4Tokens) top[threadIdx.x] = 0;
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < n * pieces; i += kQ4MulThreads) {
-            float v[8];
-            load8(i, v);
-            uint32_t big = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t b = fbits(v[e]) & 0x7fffffffu;
-                big = b < 0x7f800000u && b > big ? b : big;
-            }
-            big = __reduce_max_sync(0xffffffffu, big);
-            if (lane == 0) atomicMax(top + i / pieces, big);
-        }
-        __syncthreads();
-    }
-    for (uint32_t i = threadIdx.x; i < n * pieces; i += kQ4MulThreads) {
-        const uint32_t token = i / pieces, at = i % pieces;
-        float v[8];
-        load8(i, v);
-        float scale = 1.0f;
-        if constexpr (PARTS == 2) {
-            const int e = 127 + 14 + 127 - (int)(top[token] >> 23);  // exponent field of 2^14 / largest
-            scale = top[token] == 0 ? 1.0f : bitsf((uint32_t)(e > 254 ? 254 : e) << 23);
-            if (at == 0) up[token] = 1.0f / scale;
-        } else if (at == 0) {
-            up[token] = 1.0f;
-        }
-        float sum = 0.0f;
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float a = v[2 * e] * scale, b = v[2 * e + 1] * scale;
-            const __half2 h = __floats2half2_rn(a, b);
-            hi[e] = h2_bits(h);
-            if constexpr (PARTS == 2) {
-                const float2 f = __half22float2(h);
-                const float ra = a - f.x, rb = b - f.y;  // NaN for an infinity: the first part carries it alone
-                lo[e] = h2_bits(__floats2half2_rn(fabsf(ra) < INFINITY ? ra : 0.0f, fabsf(rb) < INFINITY ? rb : 0.0f));
-            }
-            if constexpr (kSums) sum += a + b;
-        }
-        *reinterpret_cast<uint4*>(xs + token * shape.x_row + at * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if constexpr (PARTS == 2)
-            *reinterpret_cast<uint4*>(xs + (n + token) * shape.x_row + at * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if constexpr (kSums) {  // of a group of 32: four lanes; it stands in the token's first column
+    const uint32_t pieces = w.here * 32, all = n * pieces;
+    auto hi_slot = [&](const Q4Piece& x) { return reinterpret_cast<uint4*>(sh.xs + x.token * shape.x_row + x.at * 16); };
+    auto lo_slot = [&](const Q4Piece& x) { return reinterpret_cast<uint4*>(sh.xs + (n + x.token) * shape.x_row + x.at * 16); };
+    // sum of a piece's group of 32: four adjacent lanes; it stands in the token's first column
+    auto group_sum = [&](const Q4Piece& x, float sum) {
+        if constexpr (kSums) {
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if ((at & 3u) == 0) {
-                xsum[(at >> 2) * kCols + token] = sum;
-                if constexpr (PARTS == 2) xsum[(at >> 2) * kCols + n + token] = 0.0f;
+            if ((x.at & 3u) == 0) {
+                sh.table[(x.at >> 2) * kCols + x.token] = sum;
+                if constexpr (PARTS == 2) sh.table[(x.at >> 2) * kCols + n + x.token] = 0.0f;
+            }
+        }
+    };
+    if (threadIdx.x < kQ4Tokens) {
+        sh.up[threadIdx.x] = 1.0f;
+        sh.top[threadIdx.x] = 0;
+    }
+    if constexpr (kSums) {  // columns that nobody reads
+        for (uint32_t i = threadIdx.x; i < w.here * 8 * (kCols - cols); i += kQ4MulThreads)
+            sh.table[i / (kCols - cols) * kCols + cols + i % (kCols - cols)] = 0.0f;
+    }
+    if (PARTS == 2) __syncthreads();
+    if (threadIdx.x < all) {
+        Q4Piece at{threadIdx.x / pieces, threadIdx.x % pieces};
+        for (uint32_t i = threadIdx.x; i < all; i += kQ4Batch * kQ4MulThreads) {
+            uint4 v[kQ4Batch][PARTS];
+            Q4Piece x = at;
+#pragma unroll
+            for (int u = 0; u < kQ4Batch; ++u) {
+                load_piece<PARTS == 2>(p, shape.x_vec, (uint64_t)w.first * 256 + (uint64_t)x.at * 8, x.token,
+                                       i + u * kQ4MulThreads < all, v[u]);
+                x.next(pieces);
+            }
+#pragma unroll
+            for (int u = 0; u < kQ4Batch; ++u) {
+                if (i + u * kQ4MulThreads < all) {
+                    *hi_slot(at) = v[u][0];
+                    if constexpr (PARTS == 2) {  // binary32 as it is, where its two parts will stand
+                        *lo_slot(at) = v[u][1];
+                        const uint32_t b[8] = {v[u][0].x, v[u][0].y, v[u][0].z, v[u][0].w,
+                                               v[u][1].x, v[u][1].y, v[u][1].z, v[u][1].w};
+                        const uint32_t big = __reduce_max_sync(0xffffffffu, largest_of(b));
+                        if (w.lane == 0) atomicMax(sh.top + at.token, big);
+                    } else {
+                        const uint32_t b[4] = {v[u][0].x, v[u][0].y, v[u][0].z, v[u][0].w};
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = __half22float2(bits_h2(b[e]));
+                            sum += f.x + f.y;
+                        }
+                        group_sum(at, sum);
+                    }
+                }
+                at.next(pieces);
             }
         }
     }
-    if constexpr (kSums) {
-        const uint32_t rest = kCols - cols;  // columns that nobody reads: numbers, not what lay there
-        for (uint32_t i = threadIdx.x; i < here * 8 * rest; i += kQ4MulThreads) xsum[i / rest * kCols + cols + i % rest] = 0.0f;
-    }
     __syncthreads();
+    if (PARTS == 2) {
+        if (threadIdx.x < all) {
+            Q4Piece x{threadIdx.x / pieces, threadIdx.x % pieces};
+            for (uint32_t i = threadIdx.x; i < all; i += kQ4MulThreads) {
+                const uint4 a = *hi_slot(x), b = *lo_slot(x);
+                const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                const float scale = scale_to(sh.top[x.token], 14);
+                if (x.at == 0) sh.up[x.token] = 1.0f / scale;
+                float sum = 0.0f;
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float y = bitsf(v[2 * q]) * scale, z = bitsf(v[2 * q + 1]) * scale;
+                    const __half2 h = __floats2half2_rn(y, z);
+                    const float2 f = __half22float2(h);
+                    const float ry = y - f.x, rz = z - f.y;  // NaN for an infinity: the first part carries it alone
+                    hi[q] = h2_bits(h);
+                    lo[q] = h2_bits(__floats2half2_rn(fabsf(ry) < INFINITY ? ry : 0.0f, fabsf(rz) < INFINITY ? rz : 0.0f));
+                    sum += y + z;
+                }
+                *hi_slot(x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *lo_slot(x) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                group_sum(x, sum);
+                x.next(pieces);
+            }
+        }
+        __syncthreads();
+    }
 
     // lanes of unused columns read the first one: their results are not used
+    const uint32_t g = w.lane >> 2, t = w.lane & 3u;
     const unsigned char* x_at[NT];
 #pragma unroll
-    for (int c = 0; c < NT; ++c) x_at[c] = xs + (8 * c + g < cols ? 8 * c + g : 0) * shape.x_row + t * 16;
-
+    for (int c = 0; c < NT; ++c) x_at[c] = sh.xs + (8 * c + g < cols ? 8 * c + g : 0) * shape.x_row + t * 16;
     float total[NT][4];
     auto work = [&](Q4Block<CODE>& b, uint32_t kb) {
+        const float* sums = sh.table + kb * 8 * kCols + 2 * t;
+        const uint32_t x_kb = kb * 512;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float a[2][2], c[2][2];
-            b.s.of(lane, j, a, c);
-            const uint32_t w[4] = {b.q[j].x, b.q[j].y, b.q[j].z, b.q[j].w};
-            fetch_quads(b, ahead, j);
+            b.s.of(w.lane, j, a, c);
+            const uint32_t q[4] = {b.q[j].x, b.q[j].y, b.q[j].z, b.q[j].w};
 #pragma unroll
             for (int G = 0; G < 2; ++G) {
-                const uint32_t at = (kb * 8 + j * 2 + G) * 64;
-                float acc[NT][4] = {};
                 uint32_t f[4], f2[4];
-                quants(w[2 * G], f);
-                quants(w[2 * G + 1], f2);
+                half_quants(q[2 * G], f);
+                half_quants(q[2 * G + 1], f2);
 #pragma unroll
                 for (int m = 0; m < NT; ++m) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(x_at[m] + at);
-                    mma_f16(acc[m], f, x.x, x.y);
-                    mma_f16(acc[m], f2, x.z, x.w);
+                    const uint4 x = *reinterpret_cast<const uint4*>(x_at[m] + x_kb + (j * 2 + G) * 64);
+                    float acc[4];
+                    mma_half(acc, f, x.x, x.y);
+                    mma_half_add(acc, f2, x.z, x.w);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) total[m][e] = __fmaf_rn(a[e >> 1][G], acc[m][e], total[m][e]);
+                    for (int e = 0; e < 4; ++e) total[m][e] = __fmaf_rn(a[e >> 1][G], acc[e], total[m][e]);
                     if constexpr (kSums) {
-                        const float2 s = *reinterpret_cast<const float2*>(xsum + (kb * 8 + j * 2 + G) * kCols + 8 * m + 2 * t);
+                        const float2 s = *reinterpret_cast<const float2*>(sums + (j * 2 + G) * kCols + 8 * m);
                         total[m][0] = __fmaf_rn(c[0][G], s.x, total[m][0]);
                         total[m][1] = __fmaf_rn(c[0][G], s.y, total[m][1]);
                         total[m][2] = __fmaf_rn(c[1][G], s.x, total[m][2]);
@@ -427,74 +658,191 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_mul_kernel(const Q4Matvec
                     }
                 }
             }
+            ahead.fetch_quads(b, j);
         }
-        fetch_scales(b, ahead);
-        next(ahead);
+        ahead.fetch_scales(b);
+        ahead.next();
     };
+    q4_rounds<CODE, PARTS, NT>(p, shape, w, blk, total, sh.red, sh.part, sh.up, 1.0f, work);
+}
 
-    const uint32_t values = shape.wk * PARTS, outs = shape.wr * 16 * n;  // values of a sum: a power of two, at most 32
-    auto store = [&](uint64_t tile0, uint32_t o, float y) {
-        const uint32_t row = o & 15u, token = (o >> 4) % n;
-        const uint64_t r = (tile0 + (o >> 4) / n) * 16 + row;
-        if (r >= p.rows) return;
-        char* at = p.dst + token * p.dst_st;
-        if (p.dst_f16) reinterpret_cast<__half*>(at)[r] = __float2half_rn(y);
-        else reinterpret_cast<float*>(at)[r] = y;
+// One or two tokens of binary32 or binary16 as four digits each.
+//
+// Shared memory of a column: 16 bytes for each lane t of a 64-column block, of
+// group 0 the digits of columns 8 t + (0, 2, 1, 3, 4, 6, 5, 7), then of group 1:
+// the order in which the masks leave a word's quants.  The table holds for each
+// 64-column block and t: of group 0 and 1, columns 2 t and 2 t + 1, what is
+// subtracted from the products; Q4_1 and Q4_K: then sum(x), in units of the
+// highest digit, under the token's highest digit.
+template <int CODE, bool F32>
+__global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4MatvecPlan p, const Q4Shape shape) {
+    constexpr bool kSums = CODE != kDtypeQ4_0;
+    constexpr uint32_t kTable = kSums ? 16 : 8;   // floats of a group
+    constexpr float kBase = 12582912.0f;          // 1.5 2^23
+    extern __shared__ __align__(16) unsigned char smem[];
+    const uint32_t n = (uint32_t)p.n, cols = n * 4;
+    const Q4Shared<1> sh(smem, shape, n, kTable);
+    const Q4Place w(p, shape);
+    Q4Stream<CODE> ahead(p, shape, w);
+    Q4Block<CODE> blk[2] = {};
+    if (shape.early) ahead.fill(blk);  // the previous kernel of the stream does not write the weights
+    pdl_enter();
+    if (!shape.early) ahead.fill(blk);
+
+    // ---- the digits of x
+    const uint32_t pieces = w.here * 32, all = n * pieces;
+    // digit i of a piece; the columns stand digit by digit, as parts
+    auto slot = [&](const Q4Piece& x, uint32_t i) {
+        return reinterpret_cast<uint2*>(sh.xs + (i * n + x.token) * shape.x_row + (x.at >> 3) * 64 + (x.at & 3u) * 16 + ((x.at >> 2) & 1u) * 8);
     };
-    uint32_t odd = 0;  // which of the two blocks comes next
-    for (uint32_t round = 0; round < shape.rounds; ++round) {
-        const uint64_t tile0 = ((uint64_t)round * shape.groups + group) * shape.wr;
+    // entry of (group, column) in the table
+    auto entry = [&](uint32_t group, uint32_t col) -> float& {
+        return sh.table[(group >> 1) * 2 * kTable + (col >> 1) * (kSums ? 8 : 4) + (group & 1u) * 2 + (col & 1u)];
+    };
+    if (threadIdx.x < kQ4Tokens) {
+        sh.up[threadIdx.x] = 1.0f;
+        sh.top[threadIdx.x] = 0;
+    }
+    for (uint32_t i = threadIdx.x; i < w.here * 8 * (8 - cols); i += kQ4MulThreads) {  // columns that nobody reads
+        float& e = entry(i / (8 - cols), cols + i % (8 - cols));
+        e = kBase;
+        if constexpr (kSums) (&e)[4] = 0.0f;
+    }
+    __syncthreads();
+    if (threadIdx.x < all) {
+        Q4Piece at{threadIdx.x / pieces, threadIdx.x % pieces};
+        for (uint32_t i = threadIdx.x; i < all; i += kQ4DigitBatch * kQ4MulThreads) {
+            uint4 v[kQ4DigitBatch][F32 ? 2 : 1];
+            Q4Piece x = at;
 #pragma unroll
-        for (int m = 0; m < NT; ++m) total[m][0] = total[m][1] = total[m][2] = total[m][3] = 0.0f;
-        uint32_t kb = kb0;
-        if (tile0 + wr < tiles) {
-            if (odd && kb < kb1) {
-                work(blk[1], kb++);
-                odd = 0;
+            for (int u = 0; u < kQ4DigitBatch; ++u) {
+                load_piece<F32>(p, shape.x_vec, (uint64_t)w.first * 256 + (uint64_t)x.at * 8, x.token,
+                                i + u * kQ4MulThreads < all, v[u]);
+                x.next(pieces);
             }
-            for (; kb + 2 <= kb1; kb += 2) {
-                work(blk[0], kb);
-                work(blk[1], kb + 1);
-            }
-            if (kb < kb1) {
-                work(blk[0], kb);
-                odd = 1;
-            }
-        }
-        float* mine = red + ((round & 1u) * kQ4Warps + warp) * 16 * kCols;
 #pragma unroll
-        for (int m = 0; m < NT; ++m) {
-            *reinterpret_cast<float2*>(mine + g * kCols + 8 * m + 2 * t) = make_float2(total[m][0], total[m][1]);
-            *reinterpret_cast<float2*>(mine + (g + 8) * kCols + 8 * m + 2 * t) = make_float2(total[m][2], total[m][3]);
-        }
-        __syncthreads();
-        // output o = (tile, token, row): its values are summed by `values` adjacent lanes
-        const uint32_t per = 32 / values, v = lane % values;
-        for (uint32_t base = warp * per; base < outs; base += kQ4Warps * per) {
-            const uint32_t o = base + lane / values;
-            float y = 0.0f;
-            if (o < outs) {
-                const uint32_t token = (o >> 4) % n, w = (o >> 4) / n * shape.wk + v / PARTS;
-                y = red[(((round & 1u) * kQ4Warps + w) * 16 + (o & 15u)) * kCols + (v % PARTS) * n + token];
-            }
-            for (uint32_t d = values >> 1; d > 0; d >>= 1) y += __shfl_xor_sync(0xffffffffu, y, d);
-            if (v == 0 && o < outs) {
-                y *= up[(o >> 4) % n];
-                if (shape.splits > 1) part[(round & 1u) * outs + o] = y;
-                else store(tile0, o, y);
-            }
-        }
-        if (shape.splits > 1) {
-            cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-            cluster.sync();
-            for (uint32_t o = threadIdx.x * shape.splits + rank; o < outs; o += kQ4MulThreads * shape.splits) {
-                float y = 0.0f;
-                for (uint32_t r = 0; r < shape.splits; ++r) y += cluster.map_shared_rank(part, r)[(round & 1u) * outs + o];
-                store(tile0, o, y);
+            for (int u = 0; u < kQ4DigitBatch; ++u) {
+                if (i + u * kQ4MulThreads < all) {
+                    uint32_t b[8];
+                    if constexpr (F32) {
+                        b[0] = v[u][0].x, b[1] = v[u][0].y, b[2] = v[u][0].z, b[3] = v[u][0].w;
+                        b[4] = v[u][F32].x, b[5] = v[u][F32].y, b[6] = v[u][F32].z, b[7] = v[u][F32].w;
+                    } else {
+                        const uint32_t h[4] = {v[u][0].x, v[u][0].y, v[u][0].z, v[u][0].w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = __half22float2(bits_h2(h[e]));
+                            b[2 * e] = fbits(f.x);
+                            b[2 * e + 1] = fbits(f.y);
+                        }
+                    }
+                    // binary32 as it is, where its digits will stand
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) *slot(at, e) = make_uint2(b[2 * e], b[2 * e + 1]);
+                    const uint32_t big = __reduce_max_sync(0xffffffffu, largest_of(b));
+                    if (w.lane == 0) atomicMax(sh.top + at.token, big);
+                }
+                at.next(pieces);
             }
         }
     }
-    if (shape.splits > 1) cooperative_groups::this_cluster().sync();  // the others may still read this CTA's part
+    __syncthreads();
+    if (threadIdx.x < all) {
+        Q4Piece x{threadIdx.x / pieces, threadIdx.x % pieces};
+        for (uint32_t i = threadIdx.x; i < all; i += kQ4MulThreads) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint2 b = *slot(x, e);
+                y[2 * e] = bitsf(b.x);
+                y[2 * e + 1] = bitsf(b.y);
+            }
+            const float scale = scale_to(sh.top[x.token], 29);
+            bool lost = false;  // an infinity or NaN: it takes the whole column
+            uint32_t d[8];
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                lost = lost || !(fabsf(y[e]) < INFINITY);
+                const int X = __float2int_rn(y[e] * scale);
+                if constexpr (kSums) sum += (float)X;
+                d[e] = ((uint32_t)X + 0x00808080u) ^ 0x00808080u;  // four balanced digits
+            }
+            if (x.at == 0) sh.up[x.token] = 1.0f / scale;
+            // bytes i of the columns 0, 2, 1, 3 and 4, 6, 5, 7
+            uint32_t digit[4][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t a = d[4 * h], b = d[4 * h + 2], c = d[4 * h + 1], e = d[4 * h + 3];
+                const uint32_t ab0 = __byte_perm(a, b, 0x5140), ab2 = __byte_perm(a, b, 0x7362);  // a0 b0 a1 b1, a2 b2 a3 b3
+                const uint32_t ce0 = __byte_perm(c, e, 0x5140), ce2 = __byte_perm(c, e, 0x7362);
+                digit[0][h] = __byte_perm(ab0, ce0, 0x5410);
+                digit[1][h] = __byte_perm(ab0, ce0, 0x7632);
+                digit[2][h] = __byte_perm(ab2, ce2, 0x5410);
+                digit[3][h] = __byte_perm(ab2, ce2, 0x7632);
+            }
+            if constexpr (kSums) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                *slot(x, q) = make_uint2(digit[q][0], digit[q][1]);
+                int s = __dp4a((int)digit[q][0], 0x01010101, __dp4a((int)digit[q][1], 0x01010101, 0));
+                s += __shfl_xor_sync(0xffffffffu, s, 1);
+                s += __shfl_xor_sync(0xffffffffu, s, 2);
+                if ((x.at & 3u) == 0) {
+                    float& e = entry(x.at >> 2, q * n + x.token);
+                    e = kBase + (float)(8 * s);
+                    if constexpr (kSums) (&e)[4] = q == 3 ? sum * (1.0f / 16777216.0f) : 0.0f;
+                }
+            }
+            if (__any_sync(0xffffffffu, lost) && w.lane == 0) sh.top[x.token] = 0xffffffffu;
+            x.next(pieces);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < n && sh.top[threadIdx.x] == 0xffffffffu) sh.up[threadIdx.x] = bitsf(0x7fc00000u);
+
+    const uint32_t g = w.lane >> 2, t = w.lane & 3u;
+    // lanes of unused columns read the first one: their results are not used
+    const unsigned char* x_at = sh.xs + (g < cols ? g : 0) * shape.x_row + t * 16;
+    float total[1][4];
+    auto work = [&](Q4Block<CODE>& b, uint32_t kb) {
+        const float4* table = reinterpret_cast<const float4*>(sh.table + kb * 8 * kTable) + t * (kSums ? 2 : 1);
+        const unsigned char* x_kb = x_at + kb * 256;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float a[2][2], c[2][2];
+            b.s.of(w.lane, j, a, c);
+            const uint4 x = *reinterpret_cast<const uint4*>(x_kb + j * 64);
+            const float4 base = table[j * (kSums ? 8 : 4)];
+            const uint32_t q[4] = {b.q[j].x, b.q[j].y, b.q[j].z, b.q[j].w};
+            constexpr uint32_t kMask = 0x0f0f0f0fu;
+#pragma unroll
+            for (int G = 0; G < 2; ++G) {
+                uint32_t acc[4];
+                mma_digits(acc, q[2 * G] & kMask, (q[2 * G] >> 4) & kMask, q[2 * G + 1] & kMask, (q[2 * G + 1] >> 4) & kMask,
+                           G ? x.z : x.x, G ? x.w : x.y, 0x4b400000u);
+                const float b0 = G ? base.z : base.x, b1 = G ? base.w : base.y;
+                total[0][0] = __fmaf_rn(a[0][G], bitsf(acc[0]) - b0, total[0][0]);
+                total[0][1] = __fmaf_rn(a[0][G], bitsf(acc[1]) - b1, total[0][1]);
+                total[0][2] = __fmaf_rn(a[1][G], bitsf(acc[2]) - b0, total[0][2]);
+                total[0][3] = __fmaf_rn(a[1][G], bitsf(acc[3]) - b1, total[0][3]);
+            }
+            if constexpr (kSums) {
+                const float4 s = table[j * 8 + 1];
+                total[0][0] = __fmaf_rn(c[0][1], s.z, __fmaf_rn(c[0][0], s.x, total[0][0]));
+                total[0][1] = __fmaf_rn(c[0][1], s.w, __fmaf_rn(c[0][0], s.y, total[0][1]));
+                total[0][2] = __fmaf_rn(c[1][1], s.z, __fmaf_rn(c[1][0], s.x, total[0][2]));
+                total[0][3] = __fmaf_rn(c[1][1], s.w, __fmaf_rn(c[1][0], s.y, total[0][3]));
+            }
+            ahead.fetch_quads(b, j);
+        }
+        ahead.fetch_scales(b);
+        ahead.next();
+    };
+    q4_rounds<CODE, 4, 1>(p, shape, w, blk, total, sh.red, sh.part, sh.up, 256.0f, work);
 }
 
 template <int CODE>
@@ -510,18 +858,20 @@ cudaError_t run_q4_pack(const LaunchEnv& env, const Q4PackPlan& p) {
 
 constexpr uint64_t kSharedMost = 227 * 1024;
 
-uint64_t q4_shared_bytes(const Q4Shape& s, int code, int parts, int tiles8, uint64_t n) {
-    const uint64_t cols = 8 * tiles8;
-    return 2 * kQ4Warps * 16 * cols * 4 + (s.splits > 1 ? 2 * s.wr * 16 * n * 4 : 0) + kQ4Tokens * 8 +
-           (code != kDtypeQ4_0 ? s.blocks * 8 * cols * 4 : 0) + n * parts * (uint64_t)s.x_row;
+bool q4_by_digits(const Q4MatvecPlan& p) { return p.n <= kQ4DigitTokens; }
+
+uint64_t q4_shared_bytes(const Q4Shape& s, const Q4MatvecPlan& p) {
+    const bool digits = q4_by_digits(p), sums = p.code != kDtypeQ4_0;
+    const uint64_t parts = digits ? 4 : p.x_f16 ? 1 : 2, cols = (p.n * parts + 7) / 8 * 8;
+    const uint64_t table = digits ? (sums ? 16 : 8) : sums ? cols : 0;
+    return 2 * kQ4Warps * (16 * cols + kQ4RedPad) * 4 + (s.splits > 1 ? 2 * s.wr * 16 * p.n * 4 : 0) + kQ4Tokens * 8 +
+           s.blocks * 8 * table * 4 + p.n * parts * s.x_row;
 }
 
-template <int CODE, int PARTS, int NT>
-cudaError_t run_q4_at(const LaunchEnv& env, const Q4MatvecPlan& p, const Q4Shape& shape, uint64_t smem) {
-    static DeviceFlags ready;
+cudaError_t run_q4_kernel(void (*kernel)(Q4MatvecPlan, Q4Shape), DeviceFlags& ready, const LaunchEnv& env,
+                          const Q4MatvecPlan& p, const Q4Shape& shape, uint64_t smem) {
     if (!ready.done(env.device)) {
-        const cudaError_t err = cudaFuncSetAttribute(q4_mul_kernel<CODE, PARTS, NT>,
-                                                     cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSharedMost);
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSharedMost);
         if (err != cudaSuccess) return err;
         ready.mark(env.device);
     }
@@ -538,7 +888,7 @@ cudaError_t run_q4_at(const LaunchEnv& env, const Q4MatvecPlan& p, const Q4Shape
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = shape.splits > 1 ? 2 : 1;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, q4_mul_kernel<CODE, PARTS, NT>, p, shape);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p, shape);
     if (err == cudaSuccess) ++*env.launches;
     return err;
 }
@@ -546,28 +896,32 @@ cudaError_t run_q4_at(const LaunchEnv& env, const Q4MatvecPlan& p, const Q4Shape
 // One launch: at most kQ4Tokens columns of x.
 template <int CODE>
 cudaError_t run_q4(const LaunchEnv& env, const Q4MatvecPlan& p, const Q4Shape& shape, uint64_t smem) {
-    if (p.x_f16) return run_q4_at<CODE, 1, 1>(env, p, shape, smem);
-    if (2 * p.n <= 8) return run_q4_at<CODE, 2, 1>(env, p, shape, smem);
-    return run_q4_at<CODE, 2, 2>(env, p, shape, smem);
+    static DeviceFlags ready[5];
+    if (q4_by_digits(p))
+        return p.x_f16 ? run_q4_kernel(q4_digits_kernel<CODE, false>, ready[0], env, p, shape, smem)
+                       : run_q4_kernel(q4_digits_kernel<CODE, true>, ready[1], env, p, shape, smem);
+    if (p.x_f16) return run_q4_kernel(q4_halves_kernel<CODE, 1, 1>, ready[2], env, p, shape, smem);
+    return 2 * p.n <= 8 ? run_q4_kernel(q4_halves_kernel<CODE, 2, 1>, ready[3], env, p, shape, smem)
+                        : run_q4_kernel(q4_halves_kernel<CODE, 2, 2>, ready[4], env, p, shape, smem);
 }
 
 // How k and the rows are cut; false when the columns of x do not fit.
 bool q4_shape(const LaunchEnv& env, const Q4MatvecPlan& p, Q4Shape* out, uint64_t* smem) {
-    const int parts = p.x_f16 ? 1 : 2, tiles8 = (int)((p.n * parts + 7) / 8);
     const uint64_t tiles = (p.rows + 15) / 16, k256 = (p.k + 255) / 256;
     for (uint32_t splits = 1; splits <= 8; splits *= 2) {
         Q4Shape s{};
         s.splits = splits;
         s.blocks = (uint32_t)((k256 + splits - 1) / splits);
-        s.x_row = s.blocks * 512 + 64;  // 64 mod 128: two columns' 16-byte pieces meet no bank twice
+        // 64 more than a multiple of 128: two columns' 16-byte pieces meet no bank twice
+        s.x_row = s.blocks * (q4_by_digits(p) ? 256 : 512) + 64;
         const uint64_t groups = (uint64_t)env.sm_count / splits;
         // fewest blocks one after another in a warp; a round costs a barrier
-        // and a join besides, about half a block's time
+        // and a join besides, about a quarter of a block's time
         uint64_t best = UINT64_MAX;
         for (uint32_t wk = 1; wk <= kQ4Warps; wk *= 2) {
             const uint32_t wr = kQ4Warps / wk;
             const uint64_t rounds = (tiles + groups * wr - 1) / (groups * wr), serial = (s.blocks + wk - 1) / wk;
-            const uint64_t cost = rounds * (2 * serial + 1);
+            const uint64_t cost = rounds * (4 * serial + 1);
             if (cost >= best) continue;
             best = cost;
             s.wk = wk;
@@ -575,7 +929,7 @@ bool q4_shape(const LaunchEnv& env, const Q4MatvecPlan& p, Q4Shape* out, uint64_
             s.rounds = (uint32_t)rounds;
             s.groups = (uint32_t)((tiles + rounds * wr - 1) / (rounds * wr));
         }
-        *smem = q4_shared_bytes(s, p.code, parts, tiles8, p.n);
+        *smem = q4_shared_bytes(s, p);
         *out = s;
         if (*smem <= kSharedMost) return true;
     }
@@ -615,7 +969,7 @@ cudaError_t launch_mul_mat_q4(const LaunchEnv& env, const Q4MatvecPlan& plan) {
             p.n = (p.n + 1) / 2;
         }
         shape.early = at == 0 ? early : true;  // the product before it writes no weights
-        shape.x_vec = !plan.x_f16 && ((reinterpret_cast<uintptr_t>(p.x) | (p.n > 1 ? p.x_st : 0)) & 15u) == 0;
+        shape.x_vec = ((reinterpret_cast<uintptr_t>(p.x) | (p.n > 1 ? p.x_st : 0)) & 15u) == 0;
         cudaError_t err = cudaSuccess;
         if (p.code == kDtypeQ4_0) err = run_q4<kDtypeQ4_0>(env, p, shape, smem);
         else if (p.code == kDtypeQ4_1) err = run_q4<kDtypeQ4_1>(env, p, shape, smem);
