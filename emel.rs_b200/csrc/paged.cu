@@ -183,12 +183,20 @@ __device__ __forceinline__ float rest_of(float x) {
     return fabsf(r) < INFINITY ? r : 0.0f;
 }
 
-// A position in the order of all tiles.
+// A place in the order of all tiles: sequence, key/value head, block of query
+// heads, tile.
 struct TileAt {
-    int64_t b;       // sequence
-    uint32_t unit;   // key/value head and block of query heads
-    int64_t tile;
-    int64_t first, len, tiles;  // of sequence b
+    int32_t b;
+    uint32_t kvh, block;
+    uint32_t tile, tiles;
+    int32_t first, len;  // of sequence b
+};
+
+// Two of the 16 tokens of a subtile, as a lane loads them: rows lane / 4 and 8
+// more.  page -2: no token, -1: not known.
+struct RowsAt {
+    int32_t page[2];
+    uint32_t off[2];
 };
 
 template <typename C, int PARTS, int DP>
@@ -197,46 +205,51 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     using Q = std::conditional_t<PARTS == 1, C, float>;
     constexpr int HPU = PARTS == 1 ? 16 : 8;
     constexpr int kRow = Shape::kRow, kStages = Shape::kStages;
+    constexpr int kHeadsWarp = HPU / kAttnWarps;   // query rows that a warp stages
     constexpr int kSlot = HPU * DP * 4 + HPU * 8;  // a warp's (o, m, l) in one of its own stages
     static_assert(kSlot <= Shape::kStage, "the pieces of a segment lie in one stage");
     extern __shared__ __align__(16) unsigned char smem[];
     unsigned char* q_tile = smem + kAttnWarps * kStages * Shape::kStage;
     constexpr int kQBytes = 16 * kRow * (PARTS == 3 ? 2 : 1);
     float* q_scale = reinterpret_cast<float*>(q_tile + kQBytes);           // [16]
-    uint32_t* masks = reinterpret_cast<uint32_t*>(q_scale + 16);           // [warp][stage]
+    uint2* masks = reinterpret_cast<uint2*>(q_scale + 16);                 // [warp][8]
     int64_t* shared64 = reinterpret_cast<int64_t*>(masks + kAttnWarps * 8);  // [8]
     pdl_enter();
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t g = lane >> 2, t4 = lane & 3;
-    const uint32_t blocks = (uint32_t)((p.rep + HPU - 1) / HPU);
-    const uint32_t units = (uint32_t)(p.heads / p.rep) * blocks;
-    const int64_t cap = (int64_t)(p.table_pages * p.page_size);
-    const int64_t batch = (int64_t)p.batch;
+    const uint32_t rep = (uint32_t)p.rep, d = (uint32_t)p.d, page_size = (uint32_t)p.page_size;
+    const uint32_t blocks = (rep + HPU - 1) / HPU, kv_heads = (uint32_t)p.heads / rep, units = kv_heads * blocks;
+    const int64_t cap64 = (int64_t)(p.table_pages * p.page_size);
+    const int32_t cap = cap64 < INT32_MAX ? (int32_t)cap64 : INT32_MAX;
+    const int32_t batch = (int32_t)p.batch;
 
-    auto span = [&](int64_t b, int64_t& first, int64_t& len) -> int64_t {  // tiles of sequence b
+    auto span = [&](int32_t b, int32_t& first, int32_t& len) -> uint32_t {  // tiles of sequence b
         len = p.lengths[b * p.len_st];
         len = len < 0 ? 0 : len > cap ? cap : len;
-        first = p.window && len > (int64_t)p.window ? len - (int64_t)p.window : 0;
-        return (len - first + kAttnTile - 1) / kAttnTile;
+        first = p.window && (uint64_t)len > p.window ? len - (int32_t)p.window : 0;
+        return (uint32_t)(len - first + kAttnTile - 1) / kAttnTile;
     };
 
     // ---- this CTA's run of tiles: the total first, then the place of its start
-    int64_t mine = 0, first_tiles = 0;
-    for (int64_t b = threadIdx.x; b < batch; b += kAttnThreads) {
-        int64_t f, n;
-        const int64_t tiles = span(b, f, n);
+    int64_t mine = 0;
+    uint32_t first_tiles = 0;
+    bool empty = false;
+    for (int32_t b = threadIdx.x; b < batch; b += kAttnThreads) {
+        int32_t f, n;
+        const uint32_t tiles = span(b, f, n);
         if (b < kAttnThreads) first_tiles = tiles;
         mine += tiles;
+        empty = empty || tiles == 0;
         if (blockIdx.x == 0) {
-            const int64_t raw = p.lengths[b * p.len_st];
+            const int32_t raw = p.lengths[b * p.len_st];
             if (raw < 0 || raw > cap) atomicExch(p.reject, p.reject_code);
         }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
     if (lane == 0) shared64[warp] = mine;
-    __syncthreads();
+    empty = __syncthreads_or(empty);
     int64_t total = 0;
 #pragma unroll
     for (int w = 0; w < kAttnWarps; ++w) total += shared64[w];
@@ -246,12 +259,13 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     const int64_t start = run * blockIdx.x;
     const int64_t stop = start + run < total ? start + run : total;
 
-    // sequences without tokens: zeros, spread over the CTAs
-    for (int64_t b = blockIdx.x; b < batch; b += gridDim.x) {
-        int64_t f, n;
-        if (span(b, f, n) != 0) continue;
-        for (uint64_t i = threadIdx.x; i < p.heads * p.d; i += kAttnThreads)
-            reinterpret_cast<Q*>(p.dst + (i / p.d) * p.dst_st[1] + b * p.dst_st[2])[i % p.d] = from_f32<Q>(0.0f);
+    if (empty) {  // sequences without tokens: zeros, spread over the CTAs
+        for (int32_t b = blockIdx.x; b < batch; b += gridDim.x) {
+            int32_t f, n;
+            if (span(b, f, n) != 0) continue;
+            for (uint64_t i = threadIdx.x; i < p.heads * d; i += kAttnThreads)
+                reinterpret_cast<Q*>(p.dst + (i / d) * p.dst_st[1] + b * p.dst_st[2])[i % d] = from_f32<Q>(0.0f);
+        }
     }
     if (start >= stop) return;
 
@@ -263,10 +277,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     } else {
         int64_t before = 0;
         __syncthreads();
-        for (int64_t base = 0; base < batch; base += kAttnThreads) {
-            const int64_t b = base + threadIdx.x;
-            int64_t f, n;
-            const int64_t tiles = b >= batch ? 0 : base == 0 ? first_tiles : span(b, f, n);
+        for (int32_t base = 0; base < batch; base += kAttnThreads) {
+            const int32_t b = base + threadIdx.x;
+            int32_t f, n;
+            const uint32_t tiles = b >= batch ? 0 : base == 0 ? first_tiles : span(b, f, n);
             int64_t sum = tiles;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -282,7 +296,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                 all += shared64[w];
             }
             const int64_t at = (before + sum - tiles) * units;  // first tile of sequence b
-            if (tiles > 0 && at <= start && start < at + tiles * units) {
+            if (tiles > 0 && at <= start && start < at + (int64_t)tiles * units) {
                 shared64[4] = b;
                 shared64[5] = start - at;
             }
@@ -293,19 +307,23 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     }
     __syncthreads();
     TileAt to;  // the next subtile to compute
-    to.b = shared64[4];
+    to.b = (int32_t)shared64[4];
     to.tiles = span(to.b, to.first, to.len);
     while (to.tiles == 0) to.tiles = span(++to.b, to.first, to.len);  // start == 0 only
     {
         const int64_t off = shared64[5];
-        to.unit = (uint32_t)(off / to.tiles);
-        to.tile = off % to.tiles;
+        const uint32_t unit = (uint32_t)(off / to.tiles);
+        to.tile = (uint32_t)(off % to.tiles);
+        to.kvh = unit / blocks;
+        to.block = unit % blocks;
     }
     auto advance = [&](TileAt& x) {
         if (++x.tile < x.tiles) return;
         x.tile = 0;
-        if (++x.unit < units) return;
-        x.unit = 0;
+        if (++x.block < blocks) return;
+        x.block = 0;
+        if (++x.kvh < kv_heads) return;
+        x.kvh = 0;
         do {
             if (++x.b >= batch) return;  // past the last tile: never used
             x.tiles = span(x.b, x.first, x.len);
@@ -314,46 +332,66 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
 
     // ---- the ring
     const uint32_t ring = shared_u32(smem) + warp * kStages * Shape::kStage;
-    uint32_t* my_masks = masks + warp * 8;
-    // the page of the token that this lane stands for (lanes 16.. repeat 0..15), -2: none
-    auto page_of = [&](const TileAt& x) -> int32_t {
-        const int64_t t = x.first + x.tile * kAttnTile + warp * kAttnSub + (lane & 15);
-        if (t >= x.len) return -2;
-        return p.table[(int64_t)((uint32_t)t / (uint32_t)p.page_size) * p.table_st[0] + x.b * p.table_st[1]];
-    };
-    auto issue = [&](const TileAt& x, int32_t page, int stage) {
-        const int64_t t = x.first + x.tile * kAttnTile + warp * kAttnSub + (lane & 15);
-        const bool in = page >= 0 && (uint64_t)page < p.pages;
-        if (!in && page != -2) atomicExch(p.reject, p.reject_code);
-        const uint32_t mask = __ballot_sync(0xffffffffu, in) & 0xffffu;
-        if (lane == 0) my_masks[stage] = mask;
-        const uint64_t off = in ? (uint32_t)t % (uint32_t)p.page_size : 0;
-        const uint64_t pg = in ? (uint64_t)page : 0;
-        const uint64_t h = x.unit / blocks;
-        const uint64_t ko = pg * p.k_st[3] + off * p.k_st[2], vo = pg * p.v_st[3] + off * p.v_st[2];
-        const char* kb = p.k + h * p.k_st[1];
-        const char* vb = p.v + h * p.v_st[1];
-        const uint32_t dst = ring + stage * Shape::kStage;
-        if (p.vec) {
-            constexpr int kChunks = DP / 8;
+    uint2* my_masks = masks + warp * 8;
+    auto rows_of = [&](const TileAt& x) -> RowsAt {
+        RowsAt r;
 #pragma unroll
-            for (int i = 0; i < kAttnSub * kChunks / 32; ++i) {
-                const uint32_t c = lane + 32 * i, row = c / kChunks, col = c % kChunks;
-                const uint64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
-                const bool use = ((mask >> row) & 1u) && col * 8 < p.d;
-                cp16(dst + row * kRow + col * 16, use ? kb + kr + col * 16 : p.k, use);
-                cp16(dst + kAttnSub * kRow + row * kRow + col * 16, use ? vb + vr + col * 16 : p.v, use);
+        for (int i = 0; i < 2; ++i) {
+            const int32_t t = x.first + (int32_t)(x.tile * kAttnTile) + warp * kAttnSub + (int32_t)g + 8 * i;
+            r.page[i] = -2;
+            r.off[i] = 0;
+            if (t < x.len) {
+                // t / page_size by the host's multiplier (t < 2^31)
+                const uint32_t at = (uint32_t)(((uint64_t)(uint32_t)t * p.page_mul) >> p.page_shift);
+                r.off[i] = (uint32_t)t - at * page_size;
+                r.page[i] = p.table[(int64_t)at * p.table_st[0] + (int64_t)x.b * p.table_st[1]];
+            }
+        }
+        return r;
+    };
+    // column chunks of 16 bytes of this lane: t4, t4 + 4, ...
+    constexpr int kChunks = DP / 32;
+    const uint32_t cols_in = d > t4 * 8 ? (d - t4 * 8 + 31) / 32 : 0;  // how many of them hold columns
+    const uint32_t dst_lane = g * kRow + t4 * 16;
+    auto issue = [&](const TileAt& x, const RowsAt& r, int stage) {
+        const char* kp[2];
+        const char* vp[2];
+        bool in[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            in[i] = (uint64_t)(int64_t)r.page[i] < p.pages;  // a negative page is a huge number
+            if (!in[i] && r.page[i] != -2) atomicExch(p.reject, p.reject_code);
+            const uint64_t page = in[i] ? (uint32_t)r.page[i] : 0, off = in[i] ? r.off[i] : 0;
+            kp[i] = p.k + x.kvh * p.k_st[1] + page * p.k_st[3] + off * p.k_st[2];
+            vp[i] = p.v + x.kvh * p.v_st[1] + page * p.v_st[3] + off * p.v_st[2];
+        }
+        const uint2 mask = make_uint2(__ballot_sync(0xffffffffu, in[0]), __ballot_sync(0xffffffffu, in[1]));
+        if (lane == 0) my_masks[stage] = mask;
+        if (p.vec) {
+            const uint32_t dst = ring + stage * Shape::kStage + dst_lane;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                kp[i] += t4 * 16;
+                vp[i] += t4 * 16;
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j) {
+                    const bool use = in[i] && (uint32_t)j < cols_in;
+                    cp16(dst + i * 8 * kRow + j * 64, kp[i] + j * 64, use);
+                    cp16(dst + (i * 8 + kAttnSub) * kRow + j * 64, vp[i] + j * 64, use);
+                }
             }
         } else {
-            unsigned char* out = smem + (dst - shared_u32(smem));
-            for (uint32_t row = 0; row < kAttnSub; ++row) {
-                const uint64_t kr = __shfl_sync(0xffffffffu, ko, row), vr = __shfl_sync(0xffffffffu, vo, row);
-                const bool use = (mask >> row) & 1u;
+            unsigned char* out = smem + (warp * kStages + stage) * Shape::kStage;
+            for (int row = 0; row < kAttnSub; ++row) {
+                const int from = (row & 7) * 4;
+                const uint64_t kr = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row < 8 ? kp[0] : kp[1]), from);
+                const uint64_t vr = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row < 8 ? vp[0] : vp[1]), from);
+                const bool use = ((row < 8 ? mask.x : mask.y) >> from) & 1u;
                 for (uint32_t col = lane; col < DP; col += 32) {
                     uint16_t kx = 0, vx = 0;
-                    if (use && col < p.d) {
-                        kx = reinterpret_cast<const uint16_t*>(kb + kr)[col];
-                        vx = reinterpret_cast<const uint16_t*>(vb + vr)[col];
+                    if (use && col < d) {
+                        kx = reinterpret_cast<const uint16_t*>(kr)[col];
+                        vx = reinterpret_cast<const uint16_t*>(vr)[col];
                     }
                     *reinterpret_cast<uint16_t*>(out + row * kRow + col * 2) = kx;
                     *reinterpret_cast<uint16_t*>(out + (kAttnSub + row) * kRow + col * 2) = vx;
@@ -362,17 +400,17 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         }
     };
 
-    const int64_t count = stop - start;
+    const uint32_t count = (uint32_t)(stop - start);
     TileAt ahead = to;
-    int64_t left = count;  // subtiles not issued yet
-    int into = 0;          // the stage that takes the next one
-    int32_t page = page_of(ahead);
+    uint32_t left = count;  // subtiles not issued yet
+    int into = 0;           // the stage that takes the next one
+    RowsAt rows = rows_of(ahead);
     auto issue_next = [&]() {
         if (left > 0) {
-            issue(ahead, page, into);
+            issue(ahead, rows, into);
             if (--left > 0) {
                 advance(ahead);
-                page = page_of(ahead);  // in flight until the next call
+                rows = rows_of(ahead);  // in flight until the next call
             }
         }
         into = into + 1 == kStages ? 0 : into + 1;
@@ -380,6 +418,55 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     };
 #pragma unroll 1
     for (int s = 0; s < kStages - 1; ++s) issue_next();
+
+    // ---- query rows: warp w stages rows w * kHeadsWarp ...
+    float x[kHeadsWarp][DP / 32];
+    auto load_query = [&](const TileAt& at) {
+#pragma unroll
+        for (int i = 0; i < kHeadsWarp; ++i) {
+            const uint32_t r = warp * kHeadsWarp + i, h = at.block * HPU + r;
+            const Q* row = reinterpret_cast<const Q*>(p.q + ((uint64_t)at.kvh * rep + h) * p.q_st[1] + at.b * p.q_st[2]);
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                const uint32_t col = lane + 32 * c;
+                x[i][c] = h < rep && col < d ? to_f32(row[col]) : 0.0f;
+            }
+        }
+    };
+    auto stage_query = [&]() {
+#pragma unroll
+        for (int i = 0; i < kHeadsWarp; ++i) {
+            const uint32_t r = warp * kHeadsWarp + i;
+            float up = 1.0f, down = 1.0f;
+            if constexpr (PARTS == 2) {
+                float big = 0.0f;
+#pragma unroll
+                for (int c = 0; c < DP / 32; ++c) big = fmaxf(big, fabsf(x[i][c]));
+                const uint32_t bits = __reduce_max_sync(0xffffffffu, fbits(big));
+                const int e = (int)(bits >> 23) - 127;
+                if (e < 128 && e >= -126) {
+                    down = bitsf((uint32_t)(e < 127 ? 127 - e : 1) << 23);
+                    up = 1.0f / down;
+                }
+            }
+            if (lane == 0) q_scale[r] = p.scale * kLog2e * up;
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                const uint32_t col = lane + 32 * c;
+                const float y = x[i][c] * down;
+                *reinterpret_cast<C*>(q_tile + r * kRow + col * 2) = from_f32<C>(y);
+                if constexpr (PARTS >= 2) {
+                    const float rest = rest_of<C>(y);
+                    *reinterpret_cast<C*>(q_tile + (8 + r) * kRow + col * 2) = from_f32<C>(rest);
+                    if constexpr (PARTS == 3)
+                        *reinterpret_cast<C*>(q_tile + (16 + r) * kRow + col * 2) = from_f32<C>(rest_of<C>(rest));
+                }
+            }
+        }
+    };
+    load_query(to);
+    stage_query();
+    __syncthreads();
 
     // ldmatrix addresses of this lane
     const uint32_t k_at = ((lane >> 4) * 8 + (lane & 7)) * kRow + ((lane >> 3) & 1) * 16;
@@ -390,68 +477,29 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     constexpr int kHeadsLane = PARTS == 1 ? 2 : 1;  // heads of a lane's result rows: g (and g + 8)
     float o[DP / 8][4];
     float m[kHeadsLane], l[kHeadsLane], sc[kHeadsLane];
-    bool fresh = true;  // a new segment begins
+    auto begin_segment = [&]() {
+#pragma unroll
+        for (int h = 0; h < kHeadsLane; ++h) {
+            m[h] = -INFINITY;
+            l[h] = 0.0f;
+            sc[h] = q_scale[g + 8 * h];
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    };
+    begin_segment();
     int stage = kStages - 1;
     int64_t seg_start = start;
 
 #pragma unroll 1
-    for (int64_t i = 0; i < count; ++i) {
+    for (uint32_t i = 0; i < count; ++i) {
         stage = stage + 1 == kStages ? 0 : stage + 1;
-        if (fresh) {
-            fresh = false;
-            // the unit's query rows, in parts; every warp shares them
-            const uint64_t h0 = (uint64_t)(to.unit / blocks) * p.rep + (uint64_t)(to.unit % blocks) * HPU;
-            const uint32_t nh = (uint32_t)(p.rep - (to.unit % blocks) * HPU < HPU ? p.rep - (to.unit % blocks) * HPU : HPU);
-            for (uint32_t r = warp; r < HPU; r += kAttnWarps) {
-                const Q* row = reinterpret_cast<const Q*>(p.q + (h0 + r) * p.q_st[1] + to.b * p.q_st[2]);
-                float x[DP / 32];
-                float big = 0.0f;
-#pragma unroll
-                for (int c = 0; c < DP / 32; ++c) {
-                    const uint32_t col = lane + 32 * c;
-                    x[c] = r < nh && col < p.d ? to_f32(row[col]) : 0.0f;
-                    big = fmaxf(big, fabsf(x[c]));
-                }
-                float up = 1.0f, down = 1.0f;
-                if constexpr (PARTS == 2) {
-#pragma unroll
-                    for (int s = 16; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
-                    const int e = (int)((fbits(big) >> 23) & 255u) - 127;
-                    if (big < INFINITY && e >= -126) {
-                        down = bitsf((uint32_t)(e < 127 ? 127 - e : 1) << 23);
-                        up = 1.0f / down;
-                    }
-                }
-                if (lane == 0) q_scale[r] = p.scale * kLog2e * up;
-#pragma unroll
-                for (int c = 0; c < DP / 32; ++c) {
-                    const uint32_t col = lane + 32 * c;
-                    const float y = x[c] * down;
-                    *reinterpret_cast<C*>(q_tile + r * kRow + col * 2) = from_f32<C>(y);
-                    if constexpr (PARTS >= 2) {
-                        const float rest = rest_of<C>(y);
-                        *reinterpret_cast<C*>(q_tile + (8 + r) * kRow + col * 2) = from_f32<C>(rest);
-                        if constexpr (PARTS == 3)
-                            *reinterpret_cast<C*>(q_tile + (16 + r) * kRow + col * 2) = from_f32<C>(rest_of<C>(rest));
-                    }
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int h = 0; h < kHeadsLane; ++h) {
-                m[h] = -INFINITY;
-                l[h] = 0.0f;
-                sc[h] = q_scale[g + 8 * h];
-            }
-#pragma unroll
-            for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-        }
         cp_wait<kStages - 2>();
         __syncwarp();
-        const uint32_t mask = my_masks[stage];
+        const uint2 mask = my_masks[stage];
         issue_next();  // into the stage that the previous iteration has read
         const uint32_t base = ring + stage * Shape::kStage;
-        if (mask) {
+        if ((mask.x | mask.y) != 0) {
             float s[2][4] = {}, s3[PARTS == 3 ? 2 : 1][4] = {};  // s3: the last parts, apart
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
@@ -467,31 +515,39 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                     mma16816<C>(s3[PARTS == 3 ? 1 : 0], a0, 0u, a2, 0u, b[2], b[3]);
                 }
             }
-            // weights of this lane's tokens 2 t4, 2 t4 + 1 (n = 0) and 8 + those (n = 1)
+            // scores of this lane's tokens 2 t4, 2 t4 + 1 (n = 0) and 8 + those (n = 1)
             float w[kHeadsLane][4], keep[kHeadsLane];
-            bool moved = false;
 #pragma unroll
-            for (int h = 0; h < kHeadsLane; ++h) {
-                float top = -INFINITY;
+            for (int h = 0; h < kHeadsLane; ++h)
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float x = s[n][2 * h + e];
+                        float y = s[n][2 * h + e];
                         if constexpr (PARTS >= 2) {
                             // an infinite key: the first part has its sign, a part of 0 would make it NaN
                             const float more = PARTS == 3 ? s[n][2 + e] + s3[PARTS == 3 ? n : 0][e] : s[n][2 + e];
-                            x = fabsf(x) < INFINITY ? x + more : x;
+                            y = fabsf(y) < INFINITY ? y + more : y;
                         }
-                        w[h][2 * n + e] = (mask >> (8 * n + 2 * t4 + e)) & 1u ? x : -INFINITY;
-                        top = fmaxf(top, w[h][2 * n + e]);
+                        w[h][2 * n + e] = y;
                     }
+            if ((mask.x & mask.y) != 0xffffffffu) {
+#pragma unroll
+                for (int h = 0; h < kHeadsLane; ++h)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(((e < 2 ? mask.x : mask.y) >> (8 * t4 + 4 * (e & 1))) & 1u)) w[h][e] = -INFINITY;
+            }
+            bool moved = false;
+#pragma unroll
+            for (int h = 0; h < kHeadsLane; ++h) {
+                float top = fmaxf(fmaxf(w[h][0], w[h][1]), fmaxf(w[h][2], w[h][3]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 top = fmaxf(m[h], __fmaf_rn(top, sc[h], -kWeightShift));
                 const float ref = top == -INFINITY ? 0.0f : top;  // only -inf so far: every weight is 0
-                keep[h] = m[h] == top ? 1.0f : ex2(m[h] - ref);
-                moved = moved || keep[h] != 1.0f;
+                keep[h] = ex2(m[h] - ref);
+                moved = moved || m[h] != top;
                 m[h] = top;
                 float sum = 0.0f;
 #pragma unroll
@@ -546,8 +602,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         }
 
         // ---- the end of a segment: the warps' pieces join
+        const TileAt at = to;
+        const bool more = i + 1 < count;
         __syncwarp();
-        float* piece = reinterpret_cast<float*>(smem + (warp * kStages + stage) * Shape::kStage);
+        unsigned char* own = smem + (warp * kStages + stage) * Shape::kStage;
+        float* piece = reinterpret_cast<float*>(own);
 #pragma unroll
         for (int h = 0; h < kHeadsLane; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -559,87 +618,117 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         }
 #pragma unroll
         for (int n = 0; n < DP / 8; ++n) {
-            float* at = piece + g * DP + n * 8 + 2 * t4;
+            float* spot = piece + g * DP + n * 8 + 2 * t4;
             if constexpr (PARTS == 1) {
-                *reinterpret_cast<float2*>(at) = make_float2(o[n][0], o[n][1]);
-                *reinterpret_cast<float2*>(at + 8 * DP) = make_float2(o[n][2], o[n][3]);
+                *reinterpret_cast<float2*>(spot) = make_float2(o[n][0], o[n][1]);
+                *reinterpret_cast<float2*>(spot + 8 * DP) = make_float2(o[n][2], o[n][3]);
             } else {
-                *reinterpret_cast<float2*>(at) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
+                *reinterpret_cast<float2*>(spot) = make_float2(o[n][0] + o[n][2], o[n][1] + o[n][3]);
             }
         }
+        if (more) {
+            advance(to);
+            load_query(to);  // in flight while the pieces join
+        }
         __syncthreads();
-        const uint64_t h0 = (uint64_t)(to.unit / blocks) * p.rep + (uint64_t)(to.unit % blocks) * HPU;
-        const uint32_t nh = (uint32_t)(p.rep - (to.unit % blocks) * HPU < HPU ? p.rep - (to.unit % blocks) * HPU : HPU);
-        const int64_t unit_first = start + i - to.tile, unit_last = unit_first + to.tiles - 1;  // its tiles in the order
+        const uint32_t h0 = at.block * HPU, nh = rep - h0 < HPU ? rep - h0 : HPU;
+        const int64_t unit_first = start + i - at.tile, unit_last = unit_first + at.tiles - 1;  // its tiles in the order
         const bool whole = seg_start == unit_first && unit_ends;
-        const uint32_t d = (uint32_t)p.d;
-        const uint64_t slot_floats = (uint64_t)HPU * (d + 2);
+        const uint32_t quads = (d + 3) / 4;  // four columns at a time; rows of a slot are padded to them
+        const uint64_t slot_floats = (uint64_t)HPU * (quads * 4 + 2);
+        char* out = p.dst + ((uint64_t)at.kvh * rep + h0) * p.dst_st[1] + at.b * p.dst_st[2];
+        auto write = [&](uint32_t r, uint32_t q4, const float4& v, float sum) {
+            Q* row = reinterpret_cast<Q*>(out + r * p.dst_st[1]) + q4 * 4;
+            const float y[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (q4 * 4 + c < d) row[c] = from_f32<Q>(sum == 0.0f ? 0.0f : y[c] / sum);
+        };
         float* slot = p.pieces + ((uint64_t)blockIdx.x * 2 + (seg_start == start ? 0 : 1)) * slot_floats;
         auto warp_piece = [&](int w) { return reinterpret_cast<const float*>(smem + (w * kStages + stage) * Shape::kStage); };
-        for (uint32_t e = threadIdx.x; e < nh * d; e += kAttnThreads) {
-            const uint32_t r = e / d, c = e % d;
+        for (uint32_t e = threadIdx.x; e < nh * quads; e += kAttnThreads) {
+            const uint32_t r = e / quads, q4 = e - r * quads;
             float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kAttnWarps; ++w) top = fmaxf(top, warp_piece(w)[HPU * DP + r]);
             const float ref = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f, x = 0.0f;
+            float sum = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < kAttnWarps; ++w) {
                 const float f = ex2(warp_piece(w)[HPU * DP + r] - ref);
+                const float4 y = *reinterpret_cast<const float4*>(warp_piece(w) + r * DP + q4 * 4);
                 sum = __fmaf_rn(f, warp_piece(w)[HPU * DP + HPU + r], sum);
-                x = __fmaf_rn(f, warp_piece(w)[r * DP + c], x);
+                v.x = __fmaf_rn(f, y.x, v.x);
+                v.y = __fmaf_rn(f, y.y, v.y);
+                v.z = __fmaf_rn(f, y.z, v.z);
+                v.w = __fmaf_rn(f, y.w, v.w);
             }
             if (whole) {
-                reinterpret_cast<Q*>(p.dst + (h0 + r) * p.dst_st[1] + to.b * p.dst_st[2])[c] =
-                    from_f32<Q>(sum == 0.0f ? 0.0f : x / sum);
+                write(r, q4, v, sum);
             } else {
-                __stcg(slot + r * d + c, x);
-                if (c == 0) {
-                    __stcg(slot + HPU * d + r, top);
-                    __stcg(slot + HPU * d + HPU + r, sum);
-                }
+                __stcg(reinterpret_cast<float4*>(slot + r * quads * 4) + q4, v);
+                if (q4 == 0) __stcg(reinterpret_cast<float2*>(slot + HPU * quads * 4) + r, make_float2(top, sum));
             }
         }
         if (!whole) {
-            const int64_t c0 = unit_first / run, c1 = unit_last / run;
+            const int64_t c0 = unit_first / run;
+            const uint32_t pieces = (uint32_t)(unit_last / run - c0) + 1;
             __threadfence();
             __syncthreads();
-            if (threadIdx.x == 0) {
-                const unsigned before = atomicAdd(p.tickets + c0, 1u);
-                shared64[6] = before == (unsigned)(c1 - c0);
-            }
+            if (threadIdx.x == 0) shared64[6] = atomicAdd(p.tickets + c0, 1u) == pieces - 1;
             __syncthreads();
             if (shared64[6]) {
+                // the last piece to come: all of them join, in the order of the tiles
                 __threadfence();
-                const int64_t n = c1 - c0 + 1;
-                const float* first_slot = p.pieces + ((uint64_t)c0 * 2 + (c0 * run == unit_first ? 0 : 1)) * slot_floats;
-                auto slot_of = [&](int64_t k) {
-                    return k == 0 ? first_slot : p.pieces + (uint64_t)(c0 + k) * 2 * slot_floats;
-                };
-                for (uint32_t e = threadIdx.x; e < nh * d; e += kAttnThreads) {
-                    const uint32_t r = e / d, c = e % d;
-                    float top = -INFINITY;
-#pragma unroll 4
-                    for (int64_t k = 0; k < n; ++k) top = fmaxf(top, __ldcg(slot_of(k) + HPU * d + r));
-                    const float ref = top == -INFINITY ? 0.0f : top;
-                    float sum = 0.0f, x = 0.0f;
-#pragma unroll 4
-                    for (int64_t k = 0; k < n; ++k) {
-                        const float* s = slot_of(k);
-                        const float f = ex2(__ldcg(s + HPU * d + r) - ref);
-                        sum = __fmaf_rn(f, __ldcg(s + HPU * d + HPU + r), sum);
-                        x = __fmaf_rn(f, __ldcg(s + r * d + c), x);
+                const float* slot0 = p.pieces + ((uint64_t)c0 * 2 + (c0 * run == unit_first ? 0 : 1)) * slot_floats;
+                auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : p.pieces + (uint64_t)(c0 + k) * 2 * slot_floats; };
+                // (m, l) of a batch of pieces; the query rows' shared memory holds them
+                constexpr uint32_t kBatch = kQBytes / (HPU * 8) < 64 ? kQBytes / (HPU * 8) : 64;
+                float2* ml = reinterpret_cast<float2*>(q_tile);  // [piece][HPU]
+                for (uint32_t base_e = 0; base_e < nh * quads; base_e += kAttnThreads) {
+                    const uint32_t e = base_e + threadIdx.x;
+                    const uint32_t r = e / quads, q4 = e - r * quads;
+                    const bool live = e < nh * quads;
+                    float top = -INFINITY, sum = 0.0f;
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (uint32_t k0 = 0; k0 < pieces; k0 += kBatch) {
+                        const uint32_t n = pieces - k0 < kBatch ? pieces - k0 : kBatch;
+                        __syncthreads();
+                        for (uint32_t j = threadIdx.x; j < n * nh; j += kAttnThreads) {
+                            const uint32_t k = j / nh, h = j - k * nh;
+                            ml[k * HPU + h] = __ldcg(reinterpret_cast<const float2*>(slot_of(k0 + k) + HPU * quads * 4) + h);
+                        }
+                        __syncthreads();
+                        if (!live) continue;
+                        float now = top;
+                        for (uint32_t k = 0; k < n; ++k) now = fmaxf(now, ml[k * HPU + r].x);
+                        const float ref = now == -INFINITY ? 0.0f : now, keep = ex2(top - ref);
+                        top = now;
+                        sum *= keep;
+                        v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep;
+#pragma unroll 8
+                        for (uint32_t k = 0; k < n; ++k) {
+                            const float4 y = __ldcg(reinterpret_cast<const float4*>(slot_of(k0 + k) + r * quads * 4) + q4);
+                            const float f = ex2(ml[k * HPU + r].x - ref);
+                            sum = __fmaf_rn(f, ml[k * HPU + r].y, sum);
+                            v.x = __fmaf_rn(f, y.x, v.x);
+                            v.y = __fmaf_rn(f, y.y, v.y);
+                            v.z = __fmaf_rn(f, y.z, v.z);
+                            v.w = __fmaf_rn(f, y.w, v.w);
+                        }
                     }
-                    reinterpret_cast<Q*>(p.dst + (h0 + r) * p.dst_st[1] + to.b * p.dst_st[2])[c] =
-                        from_f32<Q>(sum == 0.0f ? 0.0f : x / sum);
+                    if (live) write(r, q4, v, sum);
                 }
                 if (threadIdx.x == 0) p.tickets[c0] = 0;
+                __syncthreads();  // the query rows come back
             }
         }
-        __syncthreads();  // the pieces and the query rows may be overwritten
-        if (i + 1 < count) advance(to);
+        if (!more) break;
+        stage_query();
         seg_start = start + i + 1;
-        fresh = true;
+        __syncthreads();  // the pieces may be overwritten, the query rows are there
+        begin_segment();
     }
 }
 
@@ -659,7 +748,7 @@ cudaError_t run_attn_at(const LaunchEnv& env, PagedAttnPlan p) {
     using Shape = AttnShape<DP>;
     constexpr int HPU = PARTS == 1 ? 16 : 8;
     constexpr int kSmem = kAttnWarps * Shape::kStages * Shape::kStage + 16 * Shape::kRow * (PARTS == 3 ? 2 : 1) + 64 +
-                          kAttnWarps * 8 * 4 + 64;
+                          kAttnWarps * 8 * 8 + 64;
     static DeviceFlags ready;
     if (!ready.done(env.device)) {
         const cudaError_t err = cudaFuncSetAttribute(paged_attn_kernel<C, PARTS, DP>,
@@ -677,6 +766,11 @@ cudaError_t run_attn_at(const LaunchEnv& env, PagedAttnPlan p) {
                                    p.batch * (p.heads / p.rep) * ((p.rep + HPU - 1) / HPU);
     if (most < grid) grid = (uint64_t)most;
     p.min_run = 1;
+    // t / page_size = (t * page_mul) >> page_shift for t < 2^31: page_mul is
+    // 2^page_shift / page_size rounded up, with 2^page_shift >= 2^31 page_size
+    p.page_shift = 31;
+    while ((1ull << (p.page_shift - 31)) < p.page_size) ++p.page_shift;
+    p.page_mul = (uint64_t)((((unsigned __int128)1 << p.page_shift) + p.page_size - 1) / p.page_size);
     const cudaError_t err = launch_dependent(paged_attn_kernel<C, PARTS, DP>, dim3((unsigned)grid), dim3(kAttnThreads),
                                              kSmem, env.stream, p);
     if (err == cudaSuccess) ++*env.launches;
