@@ -1854,6 +1854,7 @@ emel_cuda_status emel_cuda_paged_attn(emel_cuda_context* ctx, void* stream, cons
     char* pieces = static_cast<char*>(ctx->workspace) + ctx->paged_offset;
     p.pieces = reinterpret_cast<float*>(pieces);
     p.tickets = reinterpret_cast<uint32_t*>(pieces + emel::paged_piece_bytes(ctx->sm_count));
+    p.fault = reinterpret_cast<uint32_t*>(static_cast<char*>(ctx->workspace) + emel::kFaultWordOffset);
     p.reject = reject_word(ctx);
     p.reject_code = EMEL_CUDA_INDEX_OUT_OF_BOUNDS;
     cudaError_t err = select_device(ctx);

@@ -254,6 +254,7 @@ struct PagedAttnPlan {
     bool vec;               // d % 8 == 0 and every cache row 16-byte aligned
     float* pieces;          // workspace: two pieces per CTA
     uint32_t* tickets;      // workspace: one per CTA, zero between calls
+    uint32_t* fault;        // set when a bounded wait expires
     uint32_t* reject;
     uint32_t reject_code;
 };

@@ -12,6 +12,7 @@
 #include "common.cuh"
 #include "launch.hpp"
 #include "pdl.cuh"
+#include "tma.cuh"
 
 namespace emel {
 
@@ -82,11 +83,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan 
 // inputs give the same bits.  The runs follow from the lengths on the device: no host
 // knows them.
 //
-// Tile.  A warp takes 16 of a tile's tokens on its own: a ring of STAGES
-// cp.async stages (16-byte chunks, rows padded by 16 bytes so that ldmatrix
-// meets no bank twice) runs ahead across the ends of units, without a block
-// barrier.  Rows outside [first, length) and the columns d .. DP are filled with zeros,
-// so what lies there never meets an operand.
+// Tile.  Four warps take 16 of a tile's tokens each; a fifth one finds the rows
+// and loads them with cp.async (16-byte chunks, four or eight lanes a row), up to
+// STAGES tiles ahead and across the ends of units; mbarriers say when a stage is
+// there and when it is free, every wait is bounded.  With the computing warps finding
+// their own rows that took 1 us a tile, more than the products; with one bulk copy for
+// each row of 256 bytes the copy engine took 36 cycles a row, twice the time of all
+// else.  Rows are padded by 16 bytes, so that ldmatrix meets no bank twice.  Tokens
+// outside [first, length) or on rejected pages and the columns d .. DP are filled with
+// zeros, so what lies there never meets an operand.  Rows that are not 16-byte
+// aligned are loaded by the computing warps, element by element.
 //
 // Products on m16n8k16: S[head, token] = Q K^T, whose result fragments are
 // the operand fragments of O[head, d] += P V.  Sixteen heads of a 16-bit
@@ -97,8 +103,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan 
 // weights; bfloat16 caches: 3 parts of 8 bits, the last one in a second
 // operand.  The tensor pipe has room for that: the added products cost nothing
 // in time.
-constexpr int kAttnWarps = 4;
-constexpr int kAttnThreads = kAttnWarps * 32;
+constexpr int kAttnWarps = 4;                      // that compute
+constexpr int kAttnConsumers = kAttnWarps * 32;
+constexpr int kAttnThreads = kAttnConsumers + 32;  // and the one that loads
 constexpr int kAttnSub = 16;                       // tokens of a warp's subtile
 constexpr int kAttnTile = kAttnSub * kAttnWarps;   // tokens of a tile
 constexpr float kLog2e = 1.4426950408889634f;
@@ -110,23 +117,25 @@ constexpr float kWeightShift = 8.0f;
 template <int DP>
 struct AttnShape {
     static constexpr int kRow = DP * 2 + 16;                    // bytes of a staged row
-    static constexpr int kStage = 2 * kAttnSub * kRow;          // K and V of a subtile
+    static constexpr int kStage = 2 * kAttnTile * kRow;         // K and V of a tile
     // stages and CTAs per SM that fill shared memory: 2 CTAs up to 128
     // columns, one above
-    static constexpr int kStages = DP == 64 ? 6 : DP == 96 ? 4 : DP == 128 ? 3 : DP == 192 ? 4 : 3;
+    static constexpr int kStages = DP == 64 ? 5 : DP == 96 ? 4 : DP == 128 ? 3 : DP == 192 ? 4 : 3;
     static constexpr int kCtas = DP <= 128 ? 2 : 1;
 };
 
-__device__ __forceinline__ uint32_t shared_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool in) {
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const char* src, bool in) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// arrives at the barrier when this thread's copies so far have landed
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// a barrier of the computing warps alone
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kAttnConsumers) : "memory"); }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -192,11 +201,10 @@ struct TileAt {
     int32_t first, len;  // of sequence b
 };
 
-// Two of the 16 tokens of a subtile, as a lane loads them: rows lane / 4 and 8
-// more.  page -2: no token, -1: not known.
-struct RowsAt {
-    int32_t page[2];
-    uint32_t off[2];
+// A token's row: its page (-2: no token, -1: not known) and place in it.
+struct RowAt {
+    int32_t page;
+    uint32_t off;
 };
 
 template <typename C, int PARTS, int DP>
@@ -206,14 +214,25 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     constexpr int HPU = PARTS == 1 ? 16 : 8;
     constexpr int kRow = Shape::kRow, kStages = Shape::kStages;
     constexpr int kHeadsWarp = HPU / kAttnWarps;   // query rows that a warp stages
-    constexpr int kSlot = HPU * DP * 4 + HPU * 8;  // a warp's (o, m, l) in one of its own stages
-    static_assert(kSlot <= Shape::kStage, "the pieces of a segment lie in one stage");
+    constexpr int kSlot = HPU * DP * 4 + HPU * 8;  // a warp's (o, m, l) at the end of a segment
+    static_assert(kAttnWarps * kSlot <= Shape::kStage, "the pieces of a segment lie in one stage");
     extern __shared__ __align__(16) unsigned char smem[];
-    unsigned char* q_tile = smem + kAttnWarps * kStages * Shape::kStage;
+    unsigned char* q_tile = smem + kStages * Shape::kStage;
     constexpr int kQBytes = 16 * kRow * (PARTS == 3 ? 2 : 1);
     float* q_scale = reinterpret_cast<float*>(q_tile + kQBytes);           // [16]
-    uint2* masks = reinterpret_cast<uint2*>(q_scale + 16);                 // [warp][8]
-    int64_t* shared64 = reinterpret_cast<int64_t*>(masks + kAttnWarps * 8);  // [8]
+    uint64_t* masks = reinterpret_cast<uint64_t*>(q_scale + 16);           // [stage]: bit t = token t is there
+    uint64_t* full = masks + kStages;                                      // [stage] barriers
+    uint64_t* free_ = full + kStages;
+    longlong2* places = reinterpret_cast<longlong2*>(smem + kStages * Shape::kStage + kQBytes + 64 + (kStages * 24 + 15) / 16 * 16);  // [kAttnTile]
+    uint32_t* joins = reinterpret_cast<uint32_t*>(places + kAttnTile);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(full + s, 33);  // every lane's copies, and the mask
+            mbar_init(free_ + s, kAttnWarps);
+        }
+        mbar_init_fence();
+    }
+    __syncthreads();
     pdl_enter();
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -231,35 +250,26 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         return (uint32_t)(len - first + kAttnTile - 1) / kAttnTile;
     };
 
-    // ---- this CTA's run of tiles: the total first, then the place of its start
-    int64_t mine = 0;
-    uint32_t first_tiles = 0;
-    bool empty = false;
-    for (int32_t b = threadIdx.x; b < batch; b += kAttnThreads) {
+    // ---- this CTA's run of tiles, found by every warp for itself
+    int64_t total = 0;
+    bool empty = false, bad = false;
+#pragma unroll 4
+    for (int32_t base = 0; base < batch; base += 32) {
+        const int32_t b = base + lane;
         int32_t f, n;
-        const uint32_t tiles = span(b, f, n);
-        if (b < kAttnThreads) first_tiles = tiles;
-        mine += tiles;
-        empty = empty || tiles == 0;
-        if (blockIdx.x == 0) {
-            const int32_t raw = p.lengths[b * p.len_st];
-            if (raw < 0 || raw > cap) atomicExch(p.reject, p.reject_code);
-        }
+        const uint32_t tiles = b < batch ? span(b, f, n) : 0;
+        total += tiles;
+        empty = empty || (b < batch && tiles == 0);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if (lane == 0) shared64[warp] = mine;
-    empty = __syncthreads_or(empty);
-    int64_t total = 0;
-#pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) total += shared64[w];
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     total *= units;
     int64_t run = (total + gridDim.x - 1) / gridDim.x;
     if (run < (int64_t)p.min_run) run = (int64_t)p.min_run;
     const int64_t start = run * blockIdx.x;
     const int64_t stop = start + run < total ? start + run : total;
 
-    if (empty) {  // sequences without tokens: zeros, spread over the CTAs
+    if (__any_sync(0xffffffffu, empty)) {  // sequences without tokens: zeros, spread over the CTAs
         for (int32_t b = blockIdx.x; b < batch; b += gridDim.x) {
             int32_t f, n;
             if (span(b, f, n) != 0) continue;
@@ -267,51 +277,40 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                 reinterpret_cast<Q*>(p.dst + (i / d) * p.dst_st[1] + b * p.dst_st[2])[i % d] = from_f32<Q>(0.0f);
         }
     }
+    if (blockIdx.x == 0) {
+        for (int32_t b = threadIdx.x; b < batch; b += kAttnThreads) {
+            const int32_t raw = p.lengths[b * p.len_st];
+            bad = bad || raw < 0 || raw > cap;
+        }
+        if (bad) atomicExch(p.reject, p.reject_code);
+    }
     if (start >= stop) return;
 
-    if (start == 0) {
-        if (threadIdx.x == 0) {
-            shared64[4] = 0;
-            shared64[5] = 0;
-        }
-    } else {
-        int64_t before = 0;
-        __syncthreads();
-        for (int32_t base = 0; base < batch; base += kAttnThreads) {
-            const int32_t b = base + threadIdx.x;
+    TileAt to;  // the next tile to load or to compute
+    {
+        int64_t before = 0;  // tiles of the sequences before `base`
+        uint32_t found = 0;
+        int32_t base = 0;
+        int64_t off = 0;
+        for (; base < batch; base += 32) {
+            const int32_t b = base + lane;
             int32_t f, n;
-            const uint32_t tiles = b >= batch ? 0 : base == 0 ? first_tiles : span(b, f, n);
-            int64_t sum = tiles;
+            const uint32_t tiles = b < batch ? span(b, f, n) : 0;
+            uint32_t sum = tiles;  // of 32 sequences: at most 2^30
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
+                const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += up;
             }
-            if (lane == 31) shared64[warp] = sum;
-            __syncthreads();
-            int64_t all = 0;
-#pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w) {
-                if (w < warp) sum += shared64[w];
-                all += shared64[w];
-            }
-            const int64_t at = (before + sum - tiles) * units;  // first tile of sequence b
-            if (tiles > 0 && at <= start && start < at + (int64_t)tiles * units) {
-                shared64[4] = b;
-                shared64[5] = start - at;
-            }
-            before += all;
-            __syncthreads();
-            if (start < before * units) break;
+            off = start - (before + sum - tiles) * units;  // from the first tile of sequence b on
+            found = __ballot_sync(0xffffffffu, off >= 0 && off < (int64_t)tiles * units);
+            if (found) break;
+            before += __shfl_sync(0xffffffffu, sum, 31);
         }
-    }
-    __syncthreads();
-    TileAt to;  // the next subtile to compute
-    to.b = (int32_t)shared64[4];
-    to.tiles = span(to.b, to.first, to.len);
-    while (to.tiles == 0) to.tiles = span(++to.b, to.first, to.len);  // start == 0 only
-    {
-        const int64_t off = shared64[5];
+        const int from = __ffs(found) - 1;
+        to.b = base + from;
+        off = __shfl_sync(0xffffffffu, off, from);
+        to.tiles = span(to.b, to.first, to.len);
         const uint32_t unit = (uint32_t)(off / to.tiles);
         to.tile = (uint32_t)(off % to.tiles);
         to.kvh = unit / blocks;
@@ -330,118 +329,113 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         } while (x.tiles == 0);
     };
 
-    // ---- the ring
-    const uint32_t ring = shared_u32(smem) + warp * kStages * Shape::kStage;
-    uint2* my_masks = masks + warp * 8;
-    auto rows_of = [&](const TileAt& x) -> RowsAt {
-        RowsAt r;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int32_t t = x.first + (int32_t)(x.tile * kAttnTile) + warp * kAttnSub + (int32_t)g + 8 * i;
-            r.page[i] = -2;
-            r.off[i] = 0;
-            if (t < x.len) {
-                // t / page_size by the host's multiplier (t < 2^31)
-                const uint32_t at = (uint32_t)(((uint64_t)(uint32_t)t * p.page_mul) >> p.page_shift);
-                r.off[i] = (uint32_t)t - at * page_size;
-                r.page[i] = p.table[(int64_t)at * p.table_st[0] + (int64_t)x.b * p.table_st[1]];
-            }
-        }
-        return r;
+    auto row_of = [&](const TileAt& x, uint32_t token) -> RowAt {
+        const int32_t t = x.first + (int32_t)(x.tile * kAttnTile + token);
+        if (t >= x.len) return RowAt{-2, 0};
+        // t / page_size by the host's multiplier (t < 2^31)
+        const uint32_t at = (uint32_t)(((uint64_t)(uint32_t)t * p.page_mul) >> p.page_shift);
+        return RowAt{p.table[(int64_t)at * p.table_st[0] + (int64_t)x.b * p.table_st[1]], (uint32_t)t - at * page_size};
     };
-    // column chunks of 16 bytes of this lane: t4, t4 + 4, ...
-    constexpr int kChunks = DP / 32;
-    const uint32_t cols_in = d > t4 * 8 ? (d - t4 * 8 + 31) / 32 : 0;  // how many of them hold columns
-    const uint32_t dst_lane = g * kRow + t4 * 16;
-    auto issue = [&](const TileAt& x, const RowsAt& r, int stage) {
-        const char* kp[2];
-        const char* vp[2];
-        bool in[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            in[i] = (uint64_t)(int64_t)r.page[i] < p.pages;  // a negative page is a huge number
-            if (!in[i] && r.page[i] != -2) atomicExch(p.reject, p.reject_code);
-            const uint64_t page = in[i] ? (uint32_t)r.page[i] : 0, off = in[i] ? r.off[i] : 0;
-            kp[i] = p.k + x.kvh * p.k_st[1] + page * p.k_st[3] + off * p.k_st[2];
-            vp[i] = p.v + x.kvh * p.v_st[1] + page * p.v_st[3] + off * p.v_st[2];
-        }
-        const uint2 mask = make_uint2(__ballot_sync(0xffffffffu, in[0]), __ballot_sync(0xffffffffu, in[1]));
-        if (lane == 0) my_masks[stage] = mask;
-        if (p.vec) {
-            const uint32_t dst = ring + stage * Shape::kStage + dst_lane;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                kp[i] += t4 * 16;
-                vp[i] += t4 * 16;
-#pragma unroll
-                for (int j = 0; j < kChunks; ++j) {
-                    const bool use = in[i] && (uint32_t)j < cols_in;
-                    cp16(dst + i * 8 * kRow + j * 64, kp[i] + j * 64, use);
-                    cp16(dst + (i * 8 + kAttnSub) * kRow + j * 64, vp[i] + j * 64, use);
-                }
-            }
-        } else {
-            unsigned char* out = smem + (warp * kStages + stage) * Shape::kStage;
-            for (int row = 0; row < kAttnSub; ++row) {
-                const int from = (row & 7) * 4;
-                const uint64_t kr = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row < 8 ? kp[0] : kp[1]), from);
-                const uint64_t vr = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row < 8 ? vp[0] : vp[1]), from);
-                const bool use = ((row < 8 ? mask.x : mask.y) >> from) & 1u;
-                for (uint32_t col = lane; col < DP; col += 32) {
-                    uint16_t kx = 0, vx = 0;
-                    if (use && col < d) {
-                        kx = reinterpret_cast<const uint16_t*>(kr)[col];
-                        vx = reinterpret_cast<const uint16_t*>(vr)[col];
-                    }
-                    *reinterpret_cast<uint16_t*>(out + row * kRow + col * 2) = kx;
-                    *reinterpret_cast<uint16_t*>(out + (kAttnSub + row) * kRow + col * 2) = vx;
-                }
-            }
-        }
+    auto known = [&](const RowAt& r) {
+        const bool in = (uint64_t)(int64_t)r.page < p.pages;  // a negative page is a huge number
+        if (!in && r.page != -2) atomicExch(p.reject, p.reject_code);
+        return in;
     };
-
+    auto key_row = [&](const TileAt& x, const RowAt& r) {
+        return p.k + x.kvh * p.k_st[1] + (uint64_t)(uint32_t)r.page * p.k_st[3] + r.off * p.k_st[2];
+    };
+    auto value_row = [&](const TileAt& x, const RowAt& r) {
+        return p.v + x.kvh * p.v_st[1] + (uint64_t)(uint32_t)r.page * p.v_st[3] + r.off * p.v_st[2];
+    };
     const uint32_t count = (uint32_t)(stop - start);
-    TileAt ahead = to;
-    uint32_t left = count;  // subtiles not issued yet
-    int into = 0;           // the stage that takes the next one
-    RowsAt rows = rows_of(ahead);
-    auto issue_next = [&]() {
-        if (left > 0) {
-            issue(ahead, rows, into);
-            if (--left > 0) {
-                advance(ahead);
-                rows = rows_of(ahead);  // in flight until the next call
+
+    // ---- the loading warp
+    if (warp == kAttnWarps) {
+        if (!p.vec) return;
+        constexpr int kLanes = DP % 64 == 0 ? 8 : 4;
+        RowAt r[2] = {row_of(to, lane), row_of(to, lane + 32)};
+        int stage = 0;
+        uint32_t turn = 0;  // how often the ring has been filled
+        for (uint32_t i = 0; i < count; ++i) {
+            const TileAt at = to;
+            const RowAt now[2] = {r[0], r[1]};
+            if (i + 1 < count) {
+                advance(to);
+                r[0] = row_of(to, lane);  // in flight during this tile
+                r[1] = row_of(to, lane + 32);
+            }
+            const bool in[2] = {known(now[0]), known(now[1])};
+            const uint32_t lo = __ballot_sync(0xffffffffu, in[0]), hi = __ballot_sync(0xffffffffu, in[1]);
+            const bool waited = turn == 0 || mbar_try(free_ + stage, (turn - 1) & 1u) || mbar_wait(free_ + stage, (turn - 1) & 1u);
+            if (!__all_sync(0xffffffffu, waited)) {
+                if (lane == 0) atomicExch(p.fault, 1u);
+                return;
+            }
+            if (lane == 0) {
+                masks[stage] = (uint64_t)hi << 32 | lo;
+                mbar_arrive(full + stage);
+            }
+            // every row's addresses, for the lanes that bring it: kLanes a row,
+            // 32 / kLanes rows at a time
+            __syncwarp();
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                places[lane + 32 * h] = make_longlong2(reinterpret_cast<int64_t>(in[h] ? key_row(at, now[h]) : p.k),
+                                                       reinterpret_cast<int64_t>(in[h] ? value_row(at, now[h]) : p.v));
+            __syncwarp();
+            const uint32_t sub = lane % kLanes, of = lane / kLanes;
+            const uint32_t dst = smem_u32(smem) + stage * Shape::kStage + of * kRow + sub * 16;
+#pragma unroll
+            for (int r = 0; r < kAttnTile; r += 32 / kLanes) {
+                const longlong2 place = places[r + of];
+                const char* k = reinterpret_cast<const char*>(place.x) + sub * 16;
+                const char* v = reinterpret_cast<const char*>(place.y) + sub * 16;
+                const bool here = ((r < 32 ? lo : hi) >> ((r + of) & 31)) & 1u;
+#pragma unroll
+                for (int j = 0; j < DP / 8 / kLanes; ++j) {
+                    const bool use = here && (sub + j * kLanes) * 8 < d;
+                    cp16(dst + r * kRow + j * kLanes * 16, k + j * kLanes * 16, use);
+                    cp16(dst + (r + kAttnTile) * kRow + j * kLanes * 16, v + j * kLanes * 16, use);
+                }
+            }
+            cp_arrive(full + stage);
+            if (++stage == kStages) {
+                stage = 0;
+                ++turn;
             }
         }
-        into = into + 1 == kStages ? 0 : into + 1;
-        cp_commit();
-    };
-#pragma unroll 1
-    for (int s = 0; s < kStages - 1; ++s) issue_next();
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        return;
+    }
 
     // ---- query rows: warp w stages rows w * kHeadsWarp ...
-    float x[kHeadsWarp][DP / 32];
+    Q x[kHeadsWarp][DP / 32];
     auto load_query = [&](const TileAt& at) {
 #pragma unroll
         for (int i = 0; i < kHeadsWarp; ++i) {
-            const uint32_t r = warp * kHeadsWarp + i, h = at.block * HPU + r;
-            const Q* row = reinterpret_cast<const Q*>(p.q + ((uint64_t)at.kvh * rep + h) * p.q_st[1] + at.b * p.q_st[2]);
+            // loads without a condition are in flight together; what has no place becomes 0 later
+            const uint32_t h = at.block * HPU + warp * kHeadsWarp + i, hh = h < rep ? h : rep - 1;
+            const Q* row = reinterpret_cast<const Q*>(p.q + ((uint64_t)at.kvh * rep + hh) * p.q_st[1] + at.b * p.q_st[2]);
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) {
                 const uint32_t col = lane + 32 * c;
-                x[i][c] = h < rep && col < d ? to_f32(row[col]) : 0.0f;
+                x[i][c] = row[col < d ? col : d - 1];
             }
         }
     };
-    auto stage_query = [&]() {
+    auto stage_query = [&](const TileAt& at) {
 #pragma unroll
         for (int i = 0; i < kHeadsWarp; ++i) {
             const uint32_t r = warp * kHeadsWarp + i;
+            const bool there = at.block * HPU + r < rep;
+            float y[DP / 32];
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) y[c] = there && lane + 32 * c < d ? to_f32(x[i][c]) : 0.0f;
             float up = 1.0f, down = 1.0f;
             if constexpr (PARTS == 2) {
                 float big = 0.0f;
 #pragma unroll
-                for (int c = 0; c < DP / 32; ++c) big = fmaxf(big, fabsf(x[i][c]));
+                for (int c = 0; c < DP / 32; ++c) big = fmaxf(big, fabsf(y[c]));
                 const uint32_t bits = __reduce_max_sync(0xffffffffu, fbits(big));
                 const int e = (int)(bits >> 23) - 127;
                 if (e < 128 && e >= -126) {
@@ -453,10 +447,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) {
                 const uint32_t col = lane + 32 * c;
-                const float y = x[i][c] * down;
-                *reinterpret_cast<C*>(q_tile + r * kRow + col * 2) = from_f32<C>(y);
+                const float z = y[c] * down;
+                *reinterpret_cast<C*>(q_tile + r * kRow + col * 2) = from_f32<C>(z);
                 if constexpr (PARTS >= 2) {
-                    const float rest = rest_of<C>(y);
+                    const float rest = rest_of<C>(z);
                     *reinterpret_cast<C*>(q_tile + (8 + r) * kRow + col * 2) = from_f32<C>(rest);
                     if constexpr (PARTS == 3)
                         *reinterpret_cast<C*>(q_tile + (16 + r) * kRow + col * 2) = from_f32<C>(rest_of<C>(rest));
@@ -465,14 +459,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         }
     };
     load_query(to);
-    stage_query();
-    __syncthreads();
+    stage_query(to);
+    consumers_sync();
 
     // ldmatrix addresses of this lane
     const uint32_t k_at = ((lane >> 4) * 8 + (lane & 7)) * kRow + ((lane >> 3) & 1) * 16;
-    const uint32_t v_at = (((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16 + kAttnSub * kRow;
-    const uint32_t q_at = shared_u32(q_tile) + (((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16;
-    const uint32_t q2_at = shared_u32(q_tile) + 16 * kRow + (lane & 7) * kRow + ((lane >> 3) & 1) * 16;
+    const uint32_t v_at = (((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16 + kAttnTile * kRow;
+    const uint32_t q_at = smem_u32(q_tile) + (((lane >> 3) & 1) * 8 + (lane & 7)) * kRow + (lane >> 4) * 16;
+    const uint32_t q2_at = smem_u32(q_tile) + 16 * kRow + (lane & 7) * kRow + ((lane >> 3) & 1) * 16;
 
     constexpr int kHeadsLane = PARTS == 1 ? 2 : 1;  // heads of a lane's result rows: g (and g + 8)
     float o[DP / 8][4];
@@ -488,18 +482,39 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
     };
     begin_segment();
-    int stage = kStages - 1;
+    int stage = 0;
+    uint32_t turn = 0;
+    bool late = false;  // a wait has expired: what follows is only the walk to the end
     int64_t seg_start = start;
 
 #pragma unroll 1
     for (uint32_t i = 0; i < count; ++i) {
-        stage = stage + 1 == kStages ? 0 : stage + 1;
-        cp_wait<kStages - 2>();
-        __syncwarp();
-        const uint2 mask = my_masks[stage];
-        issue_next();  // into the stage that the previous iteration has read
-        const uint32_t base = ring + stage * Shape::kStage;
-        if ((mask.x | mask.y) != 0) {
+        unsigned char* rows = smem + stage * Shape::kStage + warp * kAttnSub * kRow;  // this warp's keys; values kAttnTile rows on
+        uint32_t mask;  // of this warp's tokens
+        if (p.vec) {
+            if (!late && !__all_sync(0xffffffffu, mbar_try(full + stage, turn & 1u) || mbar_wait(full + stage, turn & 1u))) {
+                late = true;
+                if (lane == 0) atomicExch(p.fault, 1u);
+            }
+            mask = late ? 0u : (uint32_t)(masks[stage] >> (warp * kAttnSub)) & 0xffffu;
+        } else {
+            const RowAt r = row_of(to, warp * kAttnSub + (lane & 15));
+            const bool in = known(r);
+            mask = __ballot_sync(0xffffffffu, in) & 0xffffu;
+            const uint64_t kr = in ? reinterpret_cast<uint64_t>(key_row(to, r)) : 0, vr = in ? reinterpret_cast<uint64_t>(value_row(to, r)) : 0;
+            for (int row = 0; row < kAttnSub; ++row) {
+                const uint16_t* ks = reinterpret_cast<const uint16_t*>(__shfl_sync(0xffffffffu, kr, row));
+                const uint16_t* vs = reinterpret_cast<const uint16_t*>(__shfl_sync(0xffffffffu, vr, row));
+                for (uint32_t col = lane; col < DP; col += 32) {
+                    const bool use = ((mask >> row) & 1u) && col < d;
+                    *reinterpret_cast<uint16_t*>(rows + row * kRow + col * 2) = use ? ks[col] : (uint16_t)0;
+                    *reinterpret_cast<uint16_t*>(rows + (kAttnTile + row) * kRow + col * 2) = use ? vs[col] : (uint16_t)0;
+                }
+            }
+            __syncwarp();
+        }
+        const uint32_t base = smem_u32(rows);
+        if (mask != 0) {
             float s[2][4] = {}, s3[PARTS == 3 ? 2 : 1][4] = {};  // s3: the last parts, apart
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
@@ -531,12 +546,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                         }
                         w[h][2 * n + e] = y;
                     }
-            if ((mask.x & mask.y) != 0xffffffffu) {
+            if (mask != 0xffffu) {
 #pragma unroll
                 for (int h = 0; h < kHeadsLane; ++h)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!(((e < 2 ? mask.x : mask.y) >> (8 * t4 + 4 * (e & 1))) & 1u)) w[h][e] = -INFINITY;
+                        if (!((mask >> ((e & 2) * 4 + 2 * t4 + (e & 1))) & 1u)) w[h][e] = -INFINITY;
             }
             bool moved = false;
 #pragma unroll
@@ -596,17 +611,26 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
             }
         }
         const bool unit_ends = to.tile + 1 == to.tiles;
+        auto release = [&]() {  // the stage may be filled again
+            __syncwarp();
+            if (p.vec && lane == 0) mbar_arrive(free_ + stage);
+            if (++stage == kStages) {
+                stage = 0;
+                ++turn;
+            }
+        };
         if (!unit_ends && i + 1 < count) {
             ++to.tile;
+            release();
             continue;
         }
 
-        // ---- the end of a segment: the warps' pieces join
+        // ---- the end of a segment: the warps' pieces join, in this stage
         const TileAt at = to;
         const bool more = i + 1 < count;
-        __syncwarp();
-        unsigned char* own = smem + (warp * kStages + stage) * Shape::kStage;
-        float* piece = reinterpret_cast<float*>(own);
+        consumers_sync();  // every warp has read its rows
+        unsigned char* stage_at = smem + stage * Shape::kStage;
+        float* piece = reinterpret_cast<float*>(stage_at + warp * kSlot);
 #pragma unroll
         for (int h = 0; h < kHeadsLane; ++h) {
             l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -630,7 +654,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
             advance(to);
             load_query(to);  // in flight while the pieces join
         }
-        __syncthreads();
+        consumers_sync();
         const uint32_t h0 = at.block * HPU, nh = rep - h0 < HPU ? rep - h0 : HPU;
         const int64_t unit_first = start + i - at.tile, unit_last = unit_first + at.tiles - 1;  // its tiles in the order
         const bool whole = seg_start == unit_first && unit_ends;
@@ -645,8 +669,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                 if (q4 * 4 + c < d) row[c] = from_f32<Q>(sum == 0.0f ? 0.0f : y[c] / sum);
         };
         float* slot = p.pieces + ((uint64_t)blockIdx.x * 2 + (seg_start == start ? 0 : 1)) * slot_floats;
-        auto warp_piece = [&](int w) { return reinterpret_cast<const float*>(smem + (w * kStages + stage) * Shape::kStage); };
-        for (uint32_t e = threadIdx.x; e < nh * quads; e += kAttnThreads) {
+        auto warp_piece = [&](int w) { return reinterpret_cast<const float*>(stage_at + w * kSlot); };
+        for (uint32_t e = threadIdx.x; e < nh * quads; e += kAttnConsumers) {
             const uint32_t r = e / quads, q4 = e - r * quads;
             float top = -INFINITY;
 #pragma unroll
@@ -675,10 +699,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
             const int64_t c0 = unit_first / run;
             const uint32_t pieces = (uint32_t)(unit_last / run - c0) + 1;
             __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) shared64[6] = atomicAdd(p.tickets + c0, 1u) == pieces - 1;
-            __syncthreads();
-            if (shared64[6]) {
+            consumers_sync();
+            if (threadIdx.x == 0) *joins = atomicAdd(p.tickets + c0, 1u) == pieces - 1;
+            consumers_sync();
+            if (*joins) {
                 // the last piece to come: all of them join, in the order of the tiles
                 __threadfence();
                 const float* slot0 = p.pieces + ((uint64_t)c0 * 2 + (c0 * run == unit_first ? 0 : 1)) * slot_floats;
@@ -686,7 +710,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                 // (m, l) of a batch of pieces; the query rows' shared memory holds them
                 constexpr uint32_t kBatch = kQBytes / (HPU * 8) < 64 ? kQBytes / (HPU * 8) : 64;
                 float2* ml = reinterpret_cast<float2*>(q_tile);  // [piece][HPU]
-                for (uint32_t base_e = 0; base_e < nh * quads; base_e += kAttnThreads) {
+                for (uint32_t base_e = 0; base_e < nh * quads; base_e += kAttnConsumers) {
                     const uint32_t e = base_e + threadIdx.x;
                     const uint32_t r = e / quads, q4 = e - r * quads;
                     const bool live = e < nh * quads;
@@ -694,12 +718,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     for (uint32_t k0 = 0; k0 < pieces; k0 += kBatch) {
                         const uint32_t n = pieces - k0 < kBatch ? pieces - k0 : kBatch;
-                        __syncthreads();
-                        for (uint32_t j = threadIdx.x; j < n * nh; j += kAttnThreads) {
+                        consumers_sync();
+                        for (uint32_t j = threadIdx.x; j < n * nh; j += kAttnConsumers) {
                             const uint32_t k = j / nh, h = j - k * nh;
                             ml[k * HPU + h] = __ldcg(reinterpret_cast<const float2*>(slot_of(k0 + k) + HPU * quads * 4) + h);
                         }
-                        __syncthreads();
+                        consumers_sync();
                         if (!live) continue;
                         float now = top;
                         for (uint32_t k = 0; k < n; ++k) now = fmaxf(now, ml[k * HPU + r].x);
@@ -721,13 +745,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                     if (live) write(r, q4, v, sum);
                 }
                 if (threadIdx.x == 0) p.tickets[c0] = 0;
-                __syncthreads();  // the query rows come back
+                consumers_sync();  // the query rows come back
             }
         }
         if (!more) break;
-        stage_query();
+        stage_query(to);
         seg_start = start + i + 1;
-        __syncthreads();  // the pieces may be overwritten, the query rows are there
+        consumers_sync();  // the pieces have been read, the query rows are there
+        release();
         begin_segment();
     }
 }
@@ -747,8 +772,8 @@ template <typename C, int PARTS, int DP>
 cudaError_t run_attn_at(const LaunchEnv& env, PagedAttnPlan p) {
     using Shape = AttnShape<DP>;
     constexpr int HPU = PARTS == 1 ? 16 : 8;
-    constexpr int kSmem = kAttnWarps * Shape::kStages * Shape::kStage + 16 * Shape::kRow * (PARTS == 3 ? 2 : 1) + 64 +
-                          kAttnWarps * 8 * 8 + 64;
+    constexpr int kSmem = Shape::kStages * Shape::kStage + 16 * Shape::kRow * (PARTS == 3 ? 2 : 1) + 64 +
+                          (Shape::kStages * 24 + 15) / 16 * 16 + kAttnTile * 16 + 16;
     static DeviceFlags ready;
     if (!ready.done(env.device)) {
         const cudaError_t err = cudaFuncSetAttribute(paged_attn_kernel<C, PARTS, DP>,
