@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan 
 // inputs give the same bits.  The runs follow from the lengths on the device: no host
 // knows them.
 //
-// Tile.  Four warps take 16 of a tile's tokens each; a fifth one finds the rows
-// and loads them with cp.async (16-byte chunks, four or eight lanes a row), up to
+// Tile.  Four warps take 16 of a tile's tokens each; two more find the rows
+// and load them with cp.async (16-byte chunks, four or eight lanes a row), up to
 // STAGES tiles ahead and across the ends of units; mbarriers say when a stage is
 // there and when it is free, every wait is bounded.  With the computing warps finding
 // their own rows that took 1 us a tile, more than the products; with one bulk copy for
@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan 
 // in time.
 constexpr int kAttnWarps = 4;                      // that compute
 constexpr int kAttnConsumers = kAttnWarps * 32;
-constexpr int kAttnThreads = kAttnConsumers + 32;  // and the one that loads
+constexpr int kAttnLoaders = 2;                    // that load: 32 rows of a tile each
+constexpr int kAttnThreads = kAttnConsumers + 32 * kAttnLoaders;
 constexpr int kAttnSub = 16;                       // tokens of a warp's subtile
 constexpr int kAttnTile = kAttnSub * kAttnWarps;   // tokens of a tile
 constexpr float kLog2e = 1.4426950408889634f;
@@ -201,6 +202,11 @@ struct TileAt {
     int32_t first, len;  // of sequence b
 };
 
+// a / b of numbers that nearly always have 32 bits: a 64-bit division is a call.
+__device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {
+    return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
+}
+
 // A token's row: its page (-2: no token, -1: not known) and place in it.
 struct RowAt {
     int32_t page;
@@ -220,14 +226,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     unsigned char* q_tile = smem + kStages * Shape::kStage;
     constexpr int kQBytes = 16 * kRow * (PARTS == 3 ? 2 : 1);
     float* q_scale = reinterpret_cast<float*>(q_tile + kQBytes);           // [16]
-    uint64_t* masks = reinterpret_cast<uint64_t*>(q_scale + 16);           // [stage]: bit t = token t is there
-    uint64_t* full = masks + kStages;                                      // [stage] barriers
+    uint2* masks = reinterpret_cast<uint2*>(q_scale + 16);                 // [stage]: bit t = token t (32 + t) is there
+    uint64_t* full = reinterpret_cast<uint64_t*>(masks + kStages);         // [stage] barriers
     uint64_t* free_ = full + kStages;
     longlong2* places = reinterpret_cast<longlong2*>(smem + kStages * Shape::kStage + kQBytes + 64 + (kStages * 24 + 15) / 16 * 16);  // [kAttnTile]
     uint32_t* joins = reinterpret_cast<uint32_t*>(places + kAttnTile);
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
-            mbar_init(full + s, 33);  // every lane's copies, and the mask
+            mbar_init(full + s, kAttnLoaders * 33);  // every lane's copies, and the masks
             mbar_init(free_ + s, kAttnWarps);
         }
         mbar_init_fence();
@@ -264,7 +270,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     total *= units;
-    int64_t run = (total + gridDim.x - 1) / gridDim.x;
+    int64_t run = divided(total + gridDim.x - 1, gridDim.x);
     if (run < (int64_t)p.min_run) run = (int64_t)p.min_run;
     const int64_t start = run * blockIdx.x;
     const int64_t stop = start + run < total ? start + run : total;
@@ -311,8 +317,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         to.b = base + from;
         off = __shfl_sync(0xffffffffu, off, from);
         to.tiles = span(to.b, to.first, to.len);
-        const uint32_t unit = (uint32_t)(off / to.tiles);
-        to.tile = (uint32_t)(off % to.tiles);
+        const uint32_t unit = (uint32_t)divided(off, to.tiles);
+        to.tile = (uint32_t)(off - (int64_t)unit * to.tiles);
         to.kvh = unit / blocks;
         to.block = unit % blocks;
     }
@@ -349,48 +355,45 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     };
     const uint32_t count = (uint32_t)(stop - start);
 
-    // ---- the loading warp
-    if (warp == kAttnWarps) {
+    // ---- the loading warps
+    if (warp >= kAttnWarps) {
         if (!p.vec) return;
-        constexpr int kLanes = DP % 64 == 0 ? 8 : 4;
-        RowAt r[2] = {row_of(to, lane), row_of(to, lane + 32)};
+        constexpr int kLanes = DP % 64 == 0 ? 8 : 4;  // lanes that bring a row, 32 / kLanes rows at a time
+        const uint32_t half = warp - kAttnWarps, token = half * 32 + lane;
+        const uint32_t sub = lane % kLanes, of = lane / kLanes;
+        longlong2* my_places = places + half * 32;
+        RowAt next = row_of(to, token);
         int stage = 0;
         uint32_t turn = 0;  // how often the ring has been filled
         for (uint32_t i = 0; i < count; ++i) {
-            const TileAt at = to;
-            const RowAt now[2] = {r[0], r[1]};
+            const RowAt now = next;
+            const bool in = known(now);
+            const uint32_t mask = __ballot_sync(0xffffffffu, in);
+            // every row's addresses, for the lanes that bring it
+            __syncwarp();
+            my_places[lane] = make_longlong2(reinterpret_cast<int64_t>(in ? key_row(to, now) : p.k),
+                                             reinterpret_cast<int64_t>(in ? value_row(to, now) : p.v));
             if (i + 1 < count) {
                 advance(to);
-                r[0] = row_of(to, lane);  // in flight during this tile
-                r[1] = row_of(to, lane + 32);
+                next = row_of(to, token);  // in flight during this tile
             }
-            const bool in[2] = {known(now[0]), known(now[1])};
-            const uint32_t lo = __ballot_sync(0xffffffffu, in[0]), hi = __ballot_sync(0xffffffffu, in[1]);
             const bool waited = turn == 0 || mbar_try(free_ + stage, (turn - 1) & 1u) || mbar_wait(free_ + stage, (turn - 1) & 1u);
             if (!__all_sync(0xffffffffu, waited)) {
                 if (lane == 0) atomicExch(p.fault, 1u);
                 return;
             }
             if (lane == 0) {
-                masks[stage] = (uint64_t)hi << 32 | lo;
+                (half ? masks[stage].y : masks[stage].x) = mask;
                 mbar_arrive(full + stage);
             }
-            // every row's addresses, for the lanes that bring it: kLanes a row,
-            // 32 / kLanes rows at a time
             __syncwarp();
+            const uint32_t dst = smem_u32(smem) + stage * Shape::kStage + (half * 32 + of) * kRow + sub * 16;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                places[lane + 32 * h] = make_longlong2(reinterpret_cast<int64_t>(in[h] ? key_row(at, now[h]) : p.k),
-                                                       reinterpret_cast<int64_t>(in[h] ? value_row(at, now[h]) : p.v));
-            __syncwarp();
-            const uint32_t sub = lane % kLanes, of = lane / kLanes;
-            const uint32_t dst = smem_u32(smem) + stage * Shape::kStage + of * kRow + sub * 16;
-#pragma unroll
-            for (int r = 0; r < kAttnTile; r += 32 / kLanes) {
-                const longlong2 place = places[r + of];
+            for (int r = 0; r < 32; r += 32 / kLanes) {
+                const longlong2 place = my_places[r + of];
                 const char* k = reinterpret_cast<const char*>(place.x) + sub * 16;
                 const char* v = reinterpret_cast<const char*>(place.y) + sub * 16;
-                const bool here = ((r < 32 ? lo : hi) >> ((r + of) & 31)) & 1u;
+                const bool here = (mask >> (r + of)) & 1u;
 #pragma unroll
                 for (int j = 0; j < DP / 8 / kLanes; ++j) {
                     const bool use = here && (sub + j * kLanes) * 8 < d;
@@ -496,7 +499,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                 late = true;
                 if (lane == 0) atomicExch(p.fault, 1u);
             }
-            mask = late ? 0u : (uint32_t)(masks[stage] >> (warp * kAttnSub)) & 0xffffu;
+            mask = late ? 0u : ((warp < 2 ? masks[stage].x : masks[stage].y) >> ((warp & 1) * kAttnSub)) & 0xffffu;
         } else {
             const RowAt r = row_of(to, warp * kAttnSub + (lane & 15));
             const bool in = known(r);
@@ -696,8 +699,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
             }
         }
         if (!whole) {
-            const int64_t c0 = unit_first / run;
-            const uint32_t pieces = (uint32_t)(unit_last / run - c0) + 1;
+            const int64_t c0 = divided(unit_first, run);
+            const uint32_t pieces = (uint32_t)(divided(unit_last, run) - c0) + 1;
             __threadfence();
             consumers_sync();
             if (threadIdx.x == 0) *joins = atomicAdd(p.tickets + c0, 1u) == pieces - 1;
@@ -706,46 +709,43 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                 // the last piece to come: all of them join, in the order of the tiles
                 __threadfence();
                 const float* slot0 = p.pieces + ((uint64_t)c0 * 2 + (c0 * run == unit_first ? 0 : 1)) * slot_floats;
-                auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : p.pieces + (uint64_t)(c0 + k) * 2 * slot_floats; };
-                // (m, l) of a batch of pieces; the query rows' shared memory holds them
-                constexpr uint32_t kBatch = kQBytes / (HPU * 8) < 64 ? kQBytes / (HPU * 8) : 64;
-                float2* ml = reinterpret_cast<float2*>(q_tile);  // [piece][HPU]
-                for (uint32_t base_e = 0; base_e < nh * quads; base_e += kAttnConsumers) {
-                    const uint32_t e = base_e + threadIdx.x;
+                const float* slot1 = p.pieces + (uint64_t)c0 * 2 * slot_floats;  // of pieces 1, 2, ...: every other slot on
+                constexpr uint32_t kBatch = 16;  // pieces whose loads are in flight together
+                for (uint32_t e = threadIdx.x; e < nh * quads; e += kAttnConsumers) {
                     const uint32_t r = e / quads, q4 = e - r * quads;
-                    const bool live = e < nh * quads;
                     float top = -INFINITY, sum = 0.0f;
                     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     for (uint32_t k0 = 0; k0 < pieces; k0 += kBatch) {
-                        const uint32_t n = pieces - k0 < kBatch ? pieces - k0 : kBatch;
-                        consumers_sync();
-                        for (uint32_t j = threadIdx.x; j < n * nh; j += kAttnConsumers) {
-                            const uint32_t k = j / nh, h = j - k * nh;
-                            ml[k * HPU + h] = __ldcg(reinterpret_cast<const float2*>(slot_of(k0 + k) + HPU * quads * 4) + h);
+                        float2 ml[kBatch];
+                        float4 y[kBatch];
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            const uint32_t kk = k0 + k < pieces ? k0 + k : pieces - 1;
+                            const float* s = kk == 0 ? slot0 : slot1 + (uint64_t)kk * 2 * slot_floats;
+                            ml[k] = __ldcg(reinterpret_cast<const float2*>(s + HPU * quads * 4) + r);
+                            y[k] = __ldcg(reinterpret_cast<const float4*>(s + r * quads * 4) + q4);
                         }
-                        consumers_sync();
-                        if (!live) continue;
                         float now = top;
-                        for (uint32_t k = 0; k < n; ++k) now = fmaxf(now, ml[k * HPU + r].x);
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) now = fmaxf(now, ml[k].x);  // the last one again: no harm
                         const float ref = now == -INFINITY ? 0.0f : now, keep = ex2(top - ref);
                         top = now;
                         sum *= keep;
                         v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep;
-#pragma unroll 8
-                        for (uint32_t k = 0; k < n; ++k) {
-                            const float4 y = __ldcg(reinterpret_cast<const float4*>(slot_of(k0 + k) + r * quads * 4) + q4);
-                            const float f = ex2(ml[k * HPU + r].x - ref);
-                            sum = __fmaf_rn(f, ml[k * HPU + r].y, sum);
-                            v.x = __fmaf_rn(f, y.x, v.x);
-                            v.y = __fmaf_rn(f, y.y, v.y);
-                            v.z = __fmaf_rn(f, y.z, v.z);
-                            v.w = __fmaf_rn(f, y.w, v.w);
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k) {
+                            if (k0 + k >= pieces) break;
+                            const float f = ex2(ml[k].x - ref);
+                            sum = __fmaf_rn(f, ml[k].y, sum);
+                            v.x = __fmaf_rn(f, y[k].x, v.x);
+                            v.y = __fmaf_rn(f, y[k].y, v.y);
+                            v.z = __fmaf_rn(f, y[k].z, v.z);
+                            v.w = __fmaf_rn(f, y[k].w, v.w);
                         }
                     }
-                    if (live) write(r, q4, v, sum);
+                    write(r, q4, v, sum);
                 }
                 if (threadIdx.x == 0) p.tickets[c0] = 0;
-                consumers_sync();  // the query rows come back
             }
         }
         if (!more) break;
