@@ -253,7 +253,8 @@ struct PagedAttnPlan {
     bool q_f32, cache_bf16;
     bool vec;               // d % 8 == 0 and every cache row 16-byte aligned
     float* pieces;          // workspace: two pieces per CTA
-    uint32_t* tickets;      // workspace: one per CTA, zero between calls
+    uint32_t* tickets;      // workspace: two per piece, zero between calls
+    uint64_t slots;         // set by the launcher: pieces that fit
     uint32_t* fault;        // set when a bounded wait expires
     uint32_t* reject;
     uint32_t reject_code;

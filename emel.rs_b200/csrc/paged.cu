@@ -109,6 +109,8 @@ constexpr int kAttnLoaders = 2;                    // that load: 32 rows of a ti
 constexpr int kAttnThreads = kAttnConsumers + 32 * kAttnLoaders;
 constexpr int kAttnSub = 16;                       // tokens of a warp's subtile
 constexpr int kAttnTile = kAttnSub * kAttnWarps;   // tokens of a tile
+constexpr uint32_t kJoin = 16;                     // pieces whose loads are in flight together
+constexpr uint32_t kJoinGroup = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are held as 2^(s - m) with m 8 below the largest s (in units of
 // log 2): binary16 keeps full precision down to 2^-22 of the largest weight
@@ -257,19 +259,18 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     };
 
     // ---- this CTA's run of tiles, found by every warp for itself
-    int64_t total = 0;
+    uint32_t mine = 0;
     bool empty = false, bad = false;
 #pragma unroll 4
     for (int32_t base = 0; base < batch; base += 32) {
         const int32_t b = base + lane;
         int32_t f, n;
         const uint32_t tiles = b < batch ? span(b, f, n) : 0;
-        total += tiles;
+        mine += tiles;
         empty = empty || (b < batch && tiles == 0);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    total *= units;
+    const int64_t total = (((int64_t)__reduce_add_sync(0xffffffffu, mine >> 16) << 16) +
+                           __reduce_add_sync(0xffffffffu, mine & 0xffffu)) * units;
     int64_t run = divided(total + gridDim.x - 1, gridDim.x);
     if (run < (int64_t)p.min_run) run = (int64_t)p.min_run;
     const int64_t start = run * blockIdx.x;
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         const int64_t unit_first = start + i - at.tile, unit_last = unit_first + at.tiles - 1;  // its tiles in the order
         const bool whole = seg_start == unit_first && unit_ends;
         const uint32_t quads = (d + 3) / 4;  // four columns at a time; rows of a slot are padded to them
-        const uint64_t slot_floats = (uint64_t)HPU * (quads * 4 + 2);
+        const uint64_t slot_floats = (uint64_t)HPU * (quads * 4 + 4);  // o, (m, l), a group's (m, l)
         char* out = p.dst + ((uint64_t)at.kvh * rep + h0) * p.dst_st[1] + at.b * p.dst_st[2];
         auto write = [&](uint32_t r, uint32_t q4, const float4& v, float sum) {
             Q* row = reinterpret_cast<Q*>(out + r * p.dst_st[1]) + q4 * 4;
@@ -700,41 +701,56 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         }
         if (!whole) {
             const int64_t c0 = divided(unit_first, run);
-            const uint32_t pieces = (uint32_t)(divided(unit_last, run) - c0) + 1;
-            __threadfence();
-            consumers_sync();
-            if (threadIdx.x == 0) *joins = atomicAdd(p.tickets + c0, 1u) == pieces - 1;
-            consumers_sync();
-            if (*joins) {
-                // the last piece to come: all of them join, in the order of the tiles
+            const uint32_t pieces = (uint32_t)(divided(unit_last, run) - c0) + 1, me = (uint32_t)(blockIdx.x - c0);
+            const uint64_t slot0 = (uint64_t)c0 * 2 + (c0 * run == unit_first ? 0 : 1);  // of the unit's first piece
+            // many pieces join in two steps, eight CTAs' first: each step waits for
+            // its loads about once
+            const bool groups = pieces > kJoin;
+            const uint32_t group = groups ? me / kJoinGroup : 0;
+            const uint32_t of_group = !groups ? pieces : pieces - group * kJoinGroup < kJoinGroup ? pieces - group * kJoinGroup : kJoinGroup;
+            const uint64_t head = group == 0 ? slot0 : (uint64_t)(c0 + group * kJoinGroup) * 2;  // the group's first slot
+            auto last_of = [&](uint32_t* ticket, uint32_t n) {  // of n CTAs, the last one to come here
                 __threadfence();
-                const float* slot0 = p.pieces + ((uint64_t)c0 * 2 + (c0 * run == unit_first ? 0 : 1)) * slot_floats;
-                const float* slot1 = p.pieces + (uint64_t)c0 * 2 * slot_floats;  // of pieces 1, 2, ...: every other slot on
-                constexpr uint32_t kBatch = 16;  // pieces whose loads are in flight together
+                consumers_sync();
+                if (threadIdx.x == 0) {
+                    *joins = atomicAdd(ticket, 1u) == n - 1;
+                    if (*joins) *ticket = 0;
+                }
+                consumers_sync();
+                const bool last = *joins != 0;
+                if (last) __threadfence();
+                return last;
+            };
+            // n slots from `first` on, then every `step` slots from `base`: the (m, l) at ml
+            auto join = [&](uint64_t first, uint64_t base, uint32_t step, uint32_t n, uint32_t ml_at, auto&& done) {
+                const float* s0 = p.pieces + first * slot_floats;
+                const float* s1 = p.pieces + base * slot_floats;
                 for (uint32_t e = threadIdx.x; e < nh * quads; e += kAttnConsumers) {
                     const uint32_t r = e / quads, q4 = e - r * quads;
                     float top = -INFINITY, sum = 0.0f;
                     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (uint32_t k0 = 0; k0 < pieces; k0 += kBatch) {
-                        float2 ml[kBatch];
-                        float4 y[kBatch];
+                    for (uint32_t k0 = 0; k0 < n; k0 += kJoin) {
+                        float2 ml[kJoin];
+                        float4 y[kJoin];
 #pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k) {
-                            const uint32_t kk = k0 + k < pieces ? k0 + k : pieces - 1;
-                            const float* s = kk == 0 ? slot0 : slot1 + (uint64_t)kk * 2 * slot_floats;
-                            ml[k] = __ldcg(reinterpret_cast<const float2*>(s + HPU * quads * 4) + r);
-                            y[k] = __ldcg(reinterpret_cast<const float4*>(s + r * quads * 4) + q4);
+                        for (uint32_t k = 0; k < kJoin; ++k) {
+                            ml[k] = make_float2(-INFINITY, 0.0f);
+                            y[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (k0 + k < n) {
+                                const float* s = k0 + k == 0 ? s0 : s1 + (uint64_t)(k0 + k) * step * slot_floats;
+                                ml[k] = __ldcg(reinterpret_cast<const float2*>(s + ml_at) + r);
+                                y[k] = __ldcg(reinterpret_cast<const float4*>(s + r * quads * 4) + q4);
+                            }
                         }
                         float now = top;
 #pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k) now = fmaxf(now, ml[k].x);  // the last one again: no harm
+                        for (uint32_t k = 0; k < kJoin; ++k) now = fmaxf(now, ml[k].x);
                         const float ref = now == -INFINITY ? 0.0f : now, keep = ex2(top - ref);
                         top = now;
                         sum *= keep;
                         v.x *= keep, v.y *= keep, v.z *= keep, v.w *= keep;
 #pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k) {
-                            if (k0 + k >= pieces) break;
+                        for (uint32_t k = 0; k < kJoin; ++k) {
                             const float f = ex2(ml[k].x - ref);
                             sum = __fmaf_rn(f, ml[k].y, sum);
                             v.x = __fmaf_rn(f, y[k].x, v.x);
@@ -743,9 +759,25 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                             v.w = __fmaf_rn(f, y[k].w, v.w);
                         }
                     }
-                    write(r, q4, v, sum);
+                    done(r, q4, v, top, sum);
                 }
-                if (threadIdx.x == 0) p.tickets[c0] = 0;
+            };
+            auto finish = [&](uint32_t r, uint32_t q4, const float4& v, float, float sum) { write(r, q4, v, sum); };
+            const uint32_t ml0 = HPU * quads * 4, ml1 = ml0 + HPU * 2;  // a piece's (m, l), a group's
+            if (last_of(p.tickets + head, of_group)) {
+                if (!groups) {
+                    join(head, c0 * 2, 2, pieces, ml0, finish);
+                } else {
+                    // into the group's first slot: a thread overwrites what it alone has read
+                    join(head, (uint64_t)(c0 + group * kJoinGroup) * 2, 2, of_group, ml0,
+                         [&](uint32_t r, uint32_t q4, const float4& v, float top, float sum) {
+                             float* s = p.pieces + head * slot_floats;
+                             __stcg(reinterpret_cast<float4*>(s + r * quads * 4) + q4, v);
+                             if (q4 == 0) __stcg(reinterpret_cast<float2*>(s + ml1) + r, make_float2(top, sum));
+                         });
+                    const uint32_t all = (pieces + kJoinGroup - 1) / kJoinGroup;
+                    if (last_of(p.tickets + p.slots + slot0, all)) join(slot0, c0 * 2, 2 * kJoinGroup, all, ml1, finish);
+                }
             }
         }
         if (!more) break;
@@ -782,11 +814,11 @@ cudaError_t run_attn_at(const LaunchEnv& env, PagedAttnPlan p) {
         ready.mark(env.device);
     }
     // one wave, no more CTAs than there are tiles at most or slots for pieces
-    const uint64_t slot = (uint64_t)HPU * (p.d + 2) * 4 * 2;
+    const uint64_t slot = (uint64_t)HPU * ((p.d + 3) / 4 * 4 + 4) * 4;
     uint64_t grid = (uint64_t)env.sm_count * Shape::kCtas;
-    const uint64_t slots = paged_piece_bytes(env.sm_count) / slot, tickets = paged_tickets(env.sm_count);
-    if (grid > slots) grid = slots;
-    if (grid > tickets) grid = tickets;
+    if (grid > paged_piece_bytes(env.sm_count) / (2 * slot)) grid = paged_piece_bytes(env.sm_count) / (2 * slot);
+    p.slots = 2 * grid;
+    if (2 * p.slots > paged_tickets(env.sm_count)) return cudaErrorInvalidValue;
     const unsigned __int128 most = (unsigned __int128)((p.table_pages * p.page_size + kAttnTile - 1) / kAttnTile) *
                                    p.batch * (p.heads / p.rep) * ((p.rep + HPU - 1) / HPU);
     if (most < grid) grid = (uint64_t)most;
@@ -823,8 +855,9 @@ cudaError_t launch_paged_append(const LaunchEnv& env, const PagedAppendPlan& p) 
 // Two pieces for each CTA of the widest shape (one CTA per SM, 16 heads of
 // kPagedMaxD columns and their m and l), or for each of two CTAs per SM at
 // half the columns.
-uint64_t paged_piece_bytes(int sm_count) { return (uint64_t)sm_count * 2 * 16 * (kPagedMaxD + 4) * 4; }
-uint64_t paged_tickets(int sm_count) { return (uint64_t)sm_count * 4; }
+uint64_t paged_piece_bytes(int sm_count) { return (uint64_t)sm_count * 2 * 16 * (kPagedMaxD + 8) * 4; }
+// A ticket for each slot's group and one for each slot's unit, at two CTAs per SM.
+uint64_t paged_tickets(int sm_count) { return (uint64_t)sm_count * 8; }
 
 cudaError_t launch_paged_attn(const LaunchEnv& env, const PagedAttnPlan& p) {
     if (p.cache_bf16) return p.q_f32 ? run_attn<__nv_bfloat16, 3>(env, p) : run_attn<__nv_bfloat16, 1>(env, p);
