@@ -1712,6 +1712,13 @@ static bool views_overlap(const emel_tensor_view* a, const Checked& ca, const em
     return ranges_overlap(a->data, reach_of(a, ca), b->data, reach_of(b, cb));
 }
 
+// Every row starts on a 16-byte boundary.
+static bool rows16(const emel_tensor_view* v, const Checked& c) {
+    bool ok = aligned16(v->data);
+    for (int d = 1; d < 4; ++d) ok = ok && (v->ne[d] == 1 || c.nb[d] % 16 == 0);
+    return ok;
+}
+
 static uint32_t* reject_word(emel_cuda_context* ctx) {
     return reinterpret_cast<uint32_t*>(static_cast<char*>(ctx->workspace) + emel::kRejectWordOffset);
 }
@@ -1785,6 +1792,8 @@ emel_cuda_status emel_cuda_paged_kv_append(emel_cuda_context* ctx, void* stream,
     p.pages = key_cache->ne[3];
     p.src_f32 = key->dtype == EMEL_DTYPE_F32;
     p.cache_bf16 = key_cache->dtype == EMEL_DTYPE_BF16;
+    p.vec = p.d % 8 == 0 && p.kv_heads <= 0x7fffffffull / 32 && rows16(key, cn) && rows16(value, cw) &&
+            rows16(key_cache, ck) && rows16(value_cache, cv);
     p.reject = reject_word(ctx);
     p.reject_code = EMEL_CUDA_INDEX_OUT_OF_BOUNDS;
     cudaError_t err = select_device(ctx);
@@ -1845,11 +1854,6 @@ emel_cuda_status emel_cuda_paged_attn(emel_cuda_context* ctx, void* stream, cons
     p.scale = scale;
     p.q_f32 = query->dtype == EMEL_DTYPE_F32;
     p.cache_bf16 = key_cache->dtype == EMEL_DTYPE_BF16;
-    auto rows16 = [](const emel_tensor_view* v, const Checked& c) {
-        bool ok = aligned16(v->data);
-        for (int i = 1; i < 4; ++i) ok = ok && (v->ne[i] == 1 || c.nb[i] % 16 == 0);
-        return ok;
-    };
     p.vec = d % 8 == 0 && rows16(key_cache, ck) && rows16(value_cache, cv);
     char* pieces = static_cast<char*>(ctx->workspace) + ctx->paged_offset;
     p.pieces = reinterpret_cast<float*>(pieces);

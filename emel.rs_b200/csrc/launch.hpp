@@ -226,6 +226,7 @@ struct PagedAppendPlan {
     uint64_t k_st[4], v_st[4];
     uint64_t d, kv_heads, count, page_size, pages;
     bool src_f32, cache_bf16;
+    bool vec;               // d % 8 == 0 and every row 16-byte aligned
     uint32_t* reject;
     uint32_t reject_code;
 };

@@ -35,6 +35,98 @@ __device__ __forceinline__ T from_f32(float v) {
 constexpr int kAppendThreads = 256;
 
 // ---- append ------------------------------------------------------------------
+//
+// Bytes moved are all there is: every value is read and written once.
+
+// The page of a position and the place in it; false: skipped or rejected.
+__device__ __forceinline__ bool place_of(const PagedAppendPlan& p, int64_t pos, int64_t seq, uint64_t* page, uint64_t* off) {
+    if (pos < 0) return false;
+    const uint64_t at = (uint32_t)pos / (uint32_t)p.page_size;
+    *off = (uint32_t)pos - (uint32_t)at * (uint32_t)p.page_size;
+    int64_t pg = -1;
+    if (seq >= 0 && (uint64_t)seq < p.sequences_count && at < p.table_pages)
+        pg = p.table[(int64_t)at * p.table_st[0] + seq * p.table_st[1]];
+    if (pg < 0 || (uint64_t)pg >= p.pages) {
+        atomicExch(p.reject, p.reject_code);
+        return false;
+    }
+    *page = (uint64_t)pg;
+    return true;
+}
+
+template <typename S, typename C>
+__device__ __forceinline__ C converted(S v) {
+    if constexpr (std::is_same_v<S, C>) return v;  // bits unchanged
+    else return from_f32<C>(to_f32(v));
+}
+
+// Eight values as one 16-byte store: from 16 bytes of the cache's type, or 32
+// of binary32.
+template <typename S, typename C>
+struct AppendPiece {
+    uint4 v[sizeof(S) == 4 ? 2 : 1];
+    __device__ __forceinline__ void load(const char* p) {
+#pragma unroll
+        for (uint32_t i = 0; i < sizeof(v) / 16; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void store(char* p) const {
+        if constexpr (std::is_same_v<S, C>) {
+            *reinterpret_cast<uint4*>(p) = v[0];
+        } else {
+            const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const C lo = from_f32<C>(__uint_as_float(w[2 * i])), hi = from_f32<C>(__uint_as_float(w[2 * i + 1]));
+                o[i] = *reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+            }
+            *reinterpret_cast<uint4*>(p) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+};
+
+// Rows of whole, aligned 16-byte pieces (p.vec).  A thread keeps its piece of a
+// row and goes from row to row, kAppendRows of them in flight: three loads follow
+// one another for each (position, page, and the values beside them).
+constexpr int kAppendRows = 4;
+template <typename S, typename C>
+__global__ void __launch_bounds__(kAppendThreads) append_rows_kernel(PagedAppendPlan p, uint32_t lanes) {
+    pdl_enter();
+    const uint32_t pieces = (uint32_t)p.d / 8, per = (uint32_t)p.kv_heads * pieces;
+    const uint64_t step = (uint64_t)gridDim.x * (kAppendThreads / lanes);
+    for (uint32_t x = threadIdx.x % lanes; x < per; x += lanes) {
+        const uint32_t h = x / pieces, c = x - h * pieces;
+        const char* ks = p.key + h * p.key_st[1] + c * 8 * sizeof(S);
+        const char* vs = p.value + h * p.value_st[1] + c * 8 * sizeof(S);
+        char* kd = p.k_cache + h * p.k_st[1] + c * 16;
+        char* vd = p.v_cache + h * p.v_st[1] + c * 16;
+        for (uint64_t n0 = (uint64_t)blockIdx.x * (kAppendThreads / lanes) + threadIdx.x / lanes; n0 < p.count; n0 += step * kAppendRows) {
+            int32_t pos[kAppendRows], seq[kAppendRows];
+            AppendPiece<S, C> k[kAppendRows], v[kAppendRows];
+#pragma unroll
+            for (int u = 0; u < kAppendRows; ++u) {
+                const uint64_t n = n0 + u * step;
+                if (n < p.count) {
+                    pos[u] = p.positions[(int64_t)n * p.pos_st];
+                    seq[u] = p.sequences ? p.sequences[(int64_t)n * p.seq_st] : (int32_t)n;
+                    k[u].load(ks + n * p.key_st[2]);
+                    v[u].load(vs + n * p.value_st[2]);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAppendRows; ++u) {
+                const uint64_t n = n0 + u * step;
+                uint64_t page, off;
+                if (n < p.count && place_of(p, pos[u], seq[u], &page, &off)) {
+                    k[u].store(kd + off * p.k_st[2] + page * p.k_st[3]);
+                    v[u].store(vd + off * p.v_st[2] + page * p.v_st[3]);
+                }
+            }
+        }
+    }
+}
+
+// Anything else, value by value.
 template <typename S, typename C>
 __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan p) {
     pdl_enter();
@@ -42,28 +134,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan 
     const uint64_t total = p.count * per;
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
         const uint64_t n = i / per, h = i % per / p.d, c = i % p.d;
-        const int64_t pos = p.positions[(int64_t)n * p.pos_st];
-        if (pos < 0) continue;
-        const int64_t seq = p.sequences ? p.sequences[(int64_t)n * p.seq_st] : (int64_t)n;
-        const uint64_t page_at = (uint64_t)pos / p.page_size, off = (uint64_t)pos % p.page_size;
-        int64_t page = -1;
-        if (seq >= 0 && (uint64_t)seq < p.sequences_count && page_at < p.table_pages)
-            page = p.table[(int64_t)page_at * p.table_st[0] + seq * p.table_st[1]];
-        if (page < 0 || (uint64_t)page >= p.pages) {
-            atomicExch(p.reject, p.reject_code);
+        uint64_t page, off;
+        if (!place_of(p, p.positions[(int64_t)n * p.pos_st], p.sequences ? p.sequences[(int64_t)n * p.seq_st] : (int64_t)n, &page, &off))
             continue;
-        }
-        const char* ks = p.key + c * sizeof(S) + h * p.key_st[1] + n * p.key_st[2];
-        const char* vs = p.value + c * sizeof(S) + h * p.value_st[1] + n * p.value_st[2];
-        char* kd = p.k_cache + c * 2 + h * p.k_st[1] + off * p.k_st[2] + page * p.k_st[3];
-        char* vd = p.v_cache + c * 2 + h * p.v_st[1] + off * p.v_st[2] + page * p.v_st[3];
-        if constexpr (std::is_same_v<S, C>) {
-            *reinterpret_cast<C*>(kd) = *reinterpret_cast<const S*>(ks);
-            *reinterpret_cast<C*>(vd) = *reinterpret_cast<const S*>(vs);
-        } else {
-            *reinterpret_cast<C*>(kd) = from_f32<C>(to_f32(*reinterpret_cast<const S*>(ks)));
-            *reinterpret_cast<C*>(vd) = from_f32<C>(to_f32(*reinterpret_cast<const S*>(vs)));
-        }
+        const S* k = reinterpret_cast<const S*>(p.key + h * p.key_st[1] + n * p.key_st[2]);
+        const S* v = reinterpret_cast<const S*>(p.value + h * p.value_st[1] + n * p.value_st[2]);
+        reinterpret_cast<C*>(p.k_cache + h * p.k_st[1] + off * p.k_st[2] + page * p.k_st[3])[c] = converted<S, C>(k[c]);
+        reinterpret_cast<C*>(p.v_cache + h * p.v_st[1] + off * p.v_st[2] + page * p.v_st[3])[c] = converted<S, C>(v[c]);
     }
 }
 
@@ -111,6 +188,11 @@ constexpr int kAttnSub = 16;                       // tokens of a warp's subtile
 constexpr int kAttnTile = kAttnSub * kAttnWarps;   // tokens of a tile
 constexpr uint32_t kJoin = 16;                     // pieces whose loads are in flight together
 constexpr uint32_t kJoinGroup = 8;
+// What the end of a unit costs beside its tiles, in tiles: queries, joins and
+// fences (about 2.5 us).  Runs are cut in these terms, or the CTAs with many short
+// sequences would come last: a ragged batch of 24 sequences takes 24.5 us without
+// it, 20.2, 19.6 and 20.4 with 1, 2 and 3; one of 64 sequences 127, 123, 122 and 121.
+constexpr uint32_t kUnitCost = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 // Weights are held as 2^(s - m) with m 8 below the largest s (in units of
 // log 2): binary16 keeps full precision down to 2^-22 of the largest weight
@@ -202,6 +284,7 @@ struct TileAt {
     uint32_t kvh, block;
     uint32_t tile, tiles;
     int32_t first, len;  // of sequence b
+    int64_t at;          // in the order of all tiles and of what a unit costs besides
 };
 
 // a / b of numbers that nearly always have 32 bits: a 64-bit division is a call.
@@ -266,7 +349,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         const int32_t b = base + lane;
         int32_t f, n;
         const uint32_t tiles = b < batch ? span(b, f, n) : 0;
-        mine += tiles;
+        mine += tiles ? tiles + kUnitCost : 0;
         empty = empty || (b < batch && tiles == 0);
     }
     const int64_t total = (((int64_t)__reduce_add_sync(0xffffffffu, mine >> 16) << 16) +
@@ -302,15 +385,16 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         for (; base < batch; base += 32) {
             const int32_t b = base + lane;
             int32_t f, n;
-            const uint32_t tiles = b < batch ? span(b, f, n) : 0;
-            uint32_t sum = tiles;  // of 32 sequences: at most 2^30
+            uint32_t cost = b < batch ? span(b, f, n) : 0;
+            cost += cost ? kUnitCost : 0;
+            uint32_t sum = cost;  // of 32 sequences: at most 2^31
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t up = __shfl_up_sync(0xffffffffu, sum, o);
                 if (lane >= o) sum += up;
             }
-            off = start - (before + sum - tiles) * units;  // from the first tile of sequence b on
-            found = __ballot_sync(0xffffffffu, off >= 0 && off < (int64_t)tiles * units);
+            off = start - (before + sum - cost) * units;  // from the start of sequence b on
+            found = __ballot_sync(0xffffffffu, off >= 0 && off < (int64_t)cost * units);
             if (found) break;
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
@@ -318,13 +402,17 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         to.b = base + from;
         off = __shfl_sync(0xffffffffu, off, from);
         to.tiles = span(to.b, to.first, to.len);
-        const uint32_t unit = (uint32_t)divided(off, to.tiles);
-        to.tile = (uint32_t)(off - (int64_t)unit * to.tiles);
+        const uint32_t unit = (uint32_t)divided(off, to.tiles + kUnitCost), in = (uint32_t)(off - (int64_t)unit * (to.tiles + kUnitCost));
+        to.tile = in < kUnitCost ? 0 : in - kUnitCost;
+        to.at = in < kUnitCost ? start + kUnitCost - in : start;
         to.kvh = unit / blocks;
         to.block = unit % blocks;
     }
+    if (to.at >= stop) return;
     auto advance = [&](TileAt& x) {
+        ++x.at;
         if (++x.tile < x.tiles) return;
+        x.at += kUnitCost;
         x.tile = 0;
         if (++x.block < blocks) return;
         x.block = 0;
@@ -354,7 +442,6 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     auto value_row = [&](const TileAt& x, const RowAt& r) {
         return p.v + x.kvh * p.v_st[1] + (uint64_t)(uint32_t)r.page * p.v_st[3] + r.off * p.v_st[2];
     };
-    const uint32_t count = (uint32_t)(stop - start);
 
     // ---- the loading warps
     if (warp >= kAttnWarps) {
@@ -366,7 +453,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         RowAt next = row_of(to, token);
         int stage = 0;
         uint32_t turn = 0;  // how often the ring has been filled
-        for (uint32_t i = 0; i < count; ++i) {
+        for (bool more = true; more;) {
             const RowAt now = next;
             const bool in = known(now);
             const uint32_t mask = __ballot_sync(0xffffffffu, in);
@@ -374,10 +461,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
             __syncwarp();
             my_places[lane] = make_longlong2(reinterpret_cast<int64_t>(in ? key_row(to, now) : p.k),
                                              reinterpret_cast<int64_t>(in ? value_row(to, now) : p.v));
-            if (i + 1 < count) {
-                advance(to);
-                next = row_of(to, token);  // in flight during this tile
-            }
+            advance(to);
+            more = to.at < stop;
+            if (more) next = row_of(to, token);  // in flight during this tile
             const bool waited = turn == 0 || mbar_try(free_ + stage, (turn - 1) & 1u) || mbar_wait(free_ + stage, (turn - 1) & 1u);
             if (!__all_sync(0xffffffffu, waited)) {
                 if (lane == 0) atomicExch(p.fault, 1u);
@@ -489,10 +575,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     int stage = 0;
     uint32_t turn = 0;
     bool late = false;  // a wait has expired: what follows is only the walk to the end
-    int64_t seg_start = start;
+    bool first_segment = true;
 
 #pragma unroll 1
-    for (uint32_t i = 0; i < count; ++i) {
+    for (;;) {
         unsigned char* rows = smem + stage * Shape::kStage + warp * kAttnSub * kRow;  // this warp's keys; values kAttnTile rows on
         uint32_t mask;  // of this warp's tokens
         if (p.vec) {
@@ -623,15 +709,16 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                 ++turn;
             }
         };
-        if (!unit_ends && i + 1 < count) {
+        const bool more = to.at + 1 + (unit_ends ? kUnitCost : 0) < stop;
+        if (!unit_ends && more) {
             ++to.tile;
+            ++to.at;
             release();
             continue;
         }
 
         // ---- the end of a segment: the warps' pieces join, in this stage
         const TileAt at = to;
-        const bool more = i + 1 < count;
         consumers_sync();  // every warp has read its rows
         unsigned char* stage_at = smem + stage * Shape::kStage;
         float* piece = reinterpret_cast<float*>(stage_at + warp * kSlot);
@@ -660,8 +747,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         }
         consumers_sync();
         const uint32_t h0 = at.block * HPU, nh = rep - h0 < HPU ? rep - h0 : HPU;
-        const int64_t unit_first = start + i - at.tile, unit_last = unit_first + at.tiles - 1;  // its tiles in the order
-        const bool whole = seg_start == unit_first && unit_ends;
+        const int64_t unit_first = at.at - at.tile, unit_last = unit_first + at.tiles - 1;  // its tiles in the order
+        const bool whole = unit_first >= start && unit_ends;
         const uint32_t quads = (d + 3) / 4;  // four columns at a time; rows of a slot are padded to them
         const uint64_t slot_floats = (uint64_t)HPU * (quads * 4 + 4);  // o, (m, l), a group's (m, l)
         char* out = p.dst + ((uint64_t)at.kvh * rep + h0) * p.dst_st[1] + at.b * p.dst_st[2];
@@ -672,7 +759,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
             for (int c = 0; c < 4; ++c)
                 if (q4 * 4 + c < d) row[c] = from_f32<Q>(sum == 0.0f ? 0.0f : y[c] / sum);
         };
-        float* slot = p.pieces + ((uint64_t)blockIdx.x * 2 + (seg_start == start ? 0 : 1)) * slot_floats;
+        float* slot = p.pieces + ((uint64_t)blockIdx.x * 2 + (first_segment ? 0 : 1)) * slot_floats;
         auto warp_piece = [&](int w) { return reinterpret_cast<const float*>(stage_at + w * kSlot); };
         for (uint32_t e = threadIdx.x; e < nh * quads; e += kAttnConsumers) {
             const uint32_t r = e / quads, q4 = e - r * quads;
@@ -702,7 +789,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         if (!whole) {
             const int64_t c0 = divided(unit_first, run);
             const uint32_t pieces = (uint32_t)(divided(unit_last, run) - c0) + 1, me = (uint32_t)(blockIdx.x - c0);
-            const uint64_t slot0 = (uint64_t)c0 * 2 + (c0 * run == unit_first ? 0 : 1);  // of the unit's first piece
+            // of the unit's first piece: a CTA's first segment or its last one
+            const uint64_t slot0 = (uint64_t)c0 * 2 + (unit_first - kUnitCost <= c0 * run ? 0 : 1);
             // many pieces join in two steps, eight CTAs' first: each step waits for
             // its loads about once
             const bool groups = pieces > kJoin;
@@ -782,7 +870,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
         }
         if (!more) break;
         stage_query(to);
-        seg_start = start + i + 1;
+        first_segment = false;
         consumers_sync();  // the pieces have been read, the query rows are there
         release();
         begin_segment();
@@ -791,6 +879,17 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
 
 template <typename S, typename C>
 cudaError_t run_append(const LaunchEnv& env, const PagedAppendPlan& p) {
+    if (p.vec) {
+        // lanes of a row: a power of two, so that a thread keeps its place in every row
+        const uint64_t per = p.kv_heads * (p.d / 8);
+        uint32_t lanes = 8;
+        while (lanes < kAppendThreads && lanes < per) lanes *= 2;
+        const uint64_t rows = kAppendThreads / lanes, want = (p.count + rows - 1) / rows, cap = (uint64_t)env.sm_count * 8;
+        const cudaError_t err = launch_dependent(append_rows_kernel<S, C>, dim3((unsigned)(want < cap ? want : cap)),
+                                                 dim3(kAppendThreads), 0, env.stream, p, lanes);
+        if (err == cudaSuccess) ++*env.launches;
+        return err;
+    }
     const uint64_t total = p.count * p.d * p.kv_heads;
     const uint64_t want = (total + kAppendThreads - 1) / kAppendThreads;
     const uint64_t cap = (uint64_t)env.sm_count * 8;
