@@ -1970,7 +1970,7 @@ emel_cuda_status emel_cuda_logits_adjust(emel_cuda_context* ctx, void* stream, c
                   views_overlap(dst, cd, penalties, cp))) ||
         (bias != nullptr && views_overlap(dst, cd, bias, cb)) ||
         (allowed != nullptr && views_overlap(dst, cd, allowed, ca)) ||
-        emel::logits_blocks(vocab, rows) > 0x7fffffffull)
+        vocab > 0x7fff0000ull || emel::logits_blocks(vocab, rows) > 0x7fffffffull)
         return EMEL_CUDA_INVALID_ARGUMENT;
     emel::LogitsPlan p{};
     p.src = static_cast<const char*>(src->data);

@@ -859,7 +859,8 @@ EMEL_CUDA_API emel_cuda_status emel_cuda_mul_mat_q4(emel_cuda_context* ctx, void
  *     v = -inf where bit i % 32 of word i / 32 is 0, whatever v was.
  * Statuses: INVALID_VIEW (also a partial history), INVALID_LAYOUT,
  * SHAPE_MISMATCH, INVALID_ARGUMENT (null context, dst overlapping an input
- * otherwise than as src itself, or more than 2^31 - 1 pieces of 8192 logits). */
+ * otherwise than as src itself, more than 2^31 - 2^16 logits in a row or 2^31 - 1
+ * pieces of 4096 logits). */
 EMEL_CUDA_API emel_cuda_status emel_cuda_logits_adjust(emel_cuda_context* ctx, void* stream,
                                                        const emel_tensor_view* src, const emel_tensor_view* history,
                                                        const emel_tensor_view* history_lengths,
