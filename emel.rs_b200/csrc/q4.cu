@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackPlan p) {
 // bits (e per token and CTA: the largest finite |x| in [2^29, 2^30)), and its four
 // balanced digits to the base 256 are four columns.  A group's integer sum is exact; it
 // comes out of the product on top of the bits of 1.5 2^23, so that one
-// subtraction, of that plus 8 times the digits' sum, makes sum((q - 8) digit) a
+// addition, of minus that and 8 times the digits' sum, makes sum((q - 8) digit) a
 // binary32 number.
 //
 // More tokens (q4_halves_kernel, m16n8k16 on binary16): a mask leaves the bits
@@ -225,6 +225,28 @@ __device__ __forceinline__ void half_quants(uint32_t w, uint32_t (&a)[4]) {
     a[3] = h2_bits(__hfma2(bits_h2(mask_or<0x00f000f0u>(v, base)), b16, b72));
 }
 
+// t += a (d + b) for the two columns of rows g (a0) and g + 8 (a1), on packed
+// pairs of binary32: half the instructions (2 to 5 % of the time).
+__device__ __forceinline__ void add_scaled(float (&t)[4], float a0, float a1, const uint32_t (&d)[4], float b0, float b1) {
+    asm("{\n\t.reg .b64 x, y, b, p, q, t, u;\n\t"
+        "mov.b64 x, {%4, %5};\n\tmov.b64 y, {%6, %7};\n\tmov.b64 b, {%8, %9};\n\t"
+        "mov.b64 p, {%10, %10};\n\tmov.b64 q, {%11, %11};\n\tmov.b64 t, {%0, %1};\n\tmov.b64 u, {%2, %3};\n\t"
+        "add.rn.f32x2 x, x, b;\n\tadd.rn.f32x2 y, y, b;\n\tfma.rn.f32x2 t, p, x, t;\n\tfma.rn.f32x2 u, q, y, u;\n\t"
+        "mov.b64 {%0, %1}, t;\n\tmov.b64 {%2, %3}, u;\n\t}"
+        : "+f"(t[0]), "+f"(t[1]), "+f"(t[2]), "+f"(t[3])
+        : "r"(d[0]), "r"(d[1]), "r"(d[2]), "r"(d[3]), "f"(b0), "f"(b1), "f"(a0), "f"(a1));
+}
+
+// t += a x for the two columns of rows g (a0) and g + 8 (a1), likewise.
+__device__ __forceinline__ void add_scaled(float (&t)[4], float a0, float a1, float x0, float x1, float x2, float x3) {
+    asm("{\n\t.reg .b64 x, y, p, q, t, u;\n\t"
+        "mov.b64 x, {%4, %5};\n\tmov.b64 y, {%6, %7};\n\tmov.b64 p, {%8, %8};\n\tmov.b64 q, {%9, %9};\n\t"
+        "mov.b64 t, {%0, %1};\n\tmov.b64 u, {%2, %3};\n\tfma.rn.f32x2 t, p, x, t;\n\tfma.rn.f32x2 u, q, y, u;\n\t"
+        "mov.b64 {%0, %1}, t;\n\tmov.b64 {%2, %3}, u;\n\t}"
+        : "+f"(t[0]), "+f"(t[1]), "+f"(t[2]), "+f"(t[3])
+        : "f"(x0), "f"(x1), "f"(x2), "f"(x3), "f"(a0), "f"(a1));
+}
+
 // Scales of one 256-column block as a lane holds them: of its 64-column block
 // t, slots (row g, group 0), (g, 1), (g + 8, 0), (g + 8, 1).
 template <int CODE>
@@ -244,8 +266,24 @@ struct Q4Scales {
             }
         }
     }
+    // Q4_K: a and c of this lane's own slots, once a block (28 instructions; of
+    // every 64-column block anew they took a quarter of all)
+    __device__ __forceinline__ void own(float (&a)[4], float (&c)[4]) const {
+        if constexpr (CODE == kDtypeQ4_K) {
+            // a byte under the exponent of 2^23 is 2^23 + byte
+            const auto value = [](uint32_t b, uint32_t at) { return bitsf(__byte_perm(b, 0x4b000000u, 0x7440u + at)) - 8388608.0f; };
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const float2 de = __half22float2(bits_h2(s & 2 ? r.w : r.z));
+                const uint32_t b = s & 2 ? r.y : r.x;
+                a[s] = de.x * value(b, 2 * (s & 1));
+                c[s] = __fmaf_rn(8.0f, a[s], -de.y * value(b, 2 * (s & 1) + 1));
+            }
+        }
+    }
     // a[row half][group], c likewise (Q4_0: not used), of 64-column block j
-    __device__ __forceinline__ void of(uint32_t lane, int j, float (&a)[2][2], float (&c)[2][2]) const {
+    __device__ __forceinline__ void of(uint32_t lane, int j, const float (&own_a)[4], const float (&own_c)[4], float (&a)[2][2],
+                                       float (&c)[2][2]) const {
         const uint32_t from = (lane & 28u) | (uint32_t)j;
         if constexpr (CODE == kDtypeQ4_0) {
 #pragma unroll
@@ -263,17 +301,10 @@ struct Q4Scales {
                 c[s >> 1][s & 1] = __fmaf_rn(8.0f, f.x, f.y);
             }
         } else {
-            // a byte under the exponent of 2^23 is 2^23 + byte
-            const auto value = [](uint32_t b, uint32_t at) { return bitsf(__byte_perm(b, 0x4b000000u, 0x7440u + at)) - 8388608.0f; };
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float2 de = __half22float2(bits_h2(h ? r.w : r.z));
-                const uint32_t b = __shfl_sync(0xffffffffu, h ? r.y : r.x, from);
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    a[h][s] = de.x * value(b, 2 * s);
-                    c[h][s] = __fmaf_rn(8.0f, a[h][s], -de.y * value(b, 2 * s + 1));
-                }
+            for (int s = 0; s < 4; ++s) {
+                a[s >> 1][s & 1] = __shfl_sync(0xffffffffu, own_a[s], from);
+                c[s >> 1][s & 1] = __shfl_sync(0xffffffffu, own_c[s], from);
             }
         }
     }
@@ -631,10 +662,12 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_halves_kernel(const Q4Mat
     auto work = [&](Q4Block<CODE>& b, uint32_t kb) {
         const float* sums = sh.table + kb * 8 * kCols + 2 * t;
         const uint32_t x_kb = kb * 512;
+        float own_a[4], own_c[4];
+        b.s.own(own_a, own_c);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float a[2][2], c[2][2];
-            b.s.of(w.lane, j, a, c);
+            b.s.of(w.lane, j, own_a, own_c, a, c);
             const uint32_t q[4] = {b.q[j].x, b.q[j].y, b.q[j].z, b.q[j].w};
 #pragma unroll
             for (int G = 0; G < 2; ++G) {
@@ -647,14 +680,10 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_halves_kernel(const Q4Mat
                     float acc[4];
                     mma_half(acc, f, x.x, x.y);
                     mma_half_add(acc, f2, x.z, x.w);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) total[m][e] = __fmaf_rn(a[e >> 1][G], acc[e], total[m][e]);
+                    add_scaled(total[m], a[0][G], a[1][G], acc[0], acc[1], acc[2], acc[3]);
                     if constexpr (kSums) {
                         const float2 s = *reinterpret_cast<const float2*>(sums + (j * 2 + G) * kCols + 8 * m);
-                        total[m][0] = __fmaf_rn(c[0][G], s.x, total[m][0]);
-                        total[m][1] = __fmaf_rn(c[0][G], s.y, total[m][1]);
-                        total[m][2] = __fmaf_rn(c[1][G], s.x, total[m][2]);
-                        total[m][3] = __fmaf_rn(c[1][G], s.y, total[m][3]);
+                        add_scaled(total[m], c[0][G], c[1][G], s.x, s.y, s.x, s.y);
                     }
                 }
             }
@@ -671,8 +700,8 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_halves_kernel(const Q4Mat
 // Shared memory of a column: 16 bytes for each lane t of a 64-column block, of
 // group 0 the digits of columns 8 t + (0, 2, 1, 3, 4, 6, 5, 7), then of group 1:
 // the order in which the masks leave a word's quants.  The table holds for each
-// 64-column block and t: of group 0 and 1, columns 2 t and 2 t + 1, what is
-// subtracted from the products; Q4_1 and Q4_K: then sum(x), in units of the
+// 64-column block and t: of group 0 and 1, columns 2 t and 2 t + 1, what is added to
+// the products; Q4_1 and Q4_K: then sum(x), in units of the
 // highest digit, under the token's highest digit.
 template <int CODE, bool F32>
 __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4MatvecPlan p, const Q4Shape shape) {
@@ -705,7 +734,7 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4Mat
     }
     for (uint32_t i = threadIdx.x; i < w.here * 8 * (8 - cols); i += kQ4MulThreads) {  // columns that nobody reads
         float& e = entry(i / (8 - cols), cols + i % (8 - cols));
-        e = kBase;
+        e = -kBase;
         if constexpr (kSums) (&e)[4] = 0.0f;
     }
     __syncthreads();
@@ -793,7 +822,7 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4Mat
                 s += __shfl_xor_sync(0xffffffffu, s, 2);
                 if ((x.at & 3u) == 0) {
                     float& e = entry(x.at >> 2, q * n + x.token);
-                    e = kBase + (float)(8 * s);
+                    e = -(kBase + (float)(8 * s));
                     if constexpr (kSums) (&e)[4] = q == 3 ? sum * (1.0f / 16777216.0f) : 0.0f;
                 }
             }
@@ -811,10 +840,12 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4Mat
     auto work = [&](Q4Block<CODE>& b, uint32_t kb) {
         const float4* table = reinterpret_cast<const float4*>(sh.table + kb * 8 * kTable) + t * (kSums ? 2 : 1);
         const unsigned char* x_kb = x_at + kb * 256;
+        float own_a[4], own_c[4];
+        b.s.own(own_a, own_c);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float a[2][2], c[2][2];
-            b.s.of(w.lane, j, a, c);
+            b.s.of(w.lane, j, own_a, own_c, a, c);
             const uint4 x = *reinterpret_cast<const uint4*>(x_kb + j * 64);
             const float4 base = table[j * (kSums ? 8 : 4)];
             const uint32_t q[4] = {b.q[j].x, b.q[j].y, b.q[j].z, b.q[j].w};
@@ -824,18 +855,12 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4Mat
                 uint32_t acc[4];
                 mma_digits(acc, q[2 * G] & kMask, (q[2 * G] >> 4) & kMask, q[2 * G + 1] & kMask, (q[2 * G + 1] >> 4) & kMask,
                            G ? x.z : x.x, G ? x.w : x.y, 0x4b400000u);
-                const float b0 = G ? base.z : base.x, b1 = G ? base.w : base.y;
-                total[0][0] = __fmaf_rn(a[0][G], bitsf(acc[0]) - b0, total[0][0]);
-                total[0][1] = __fmaf_rn(a[0][G], bitsf(acc[1]) - b1, total[0][1]);
-                total[0][2] = __fmaf_rn(a[1][G], bitsf(acc[2]) - b0, total[0][2]);
-                total[0][3] = __fmaf_rn(a[1][G], bitsf(acc[3]) - b1, total[0][3]);
+                add_scaled(total[0], a[0][G], a[1][G], acc, G ? base.z : base.x, G ? base.w : base.y);
             }
             if constexpr (kSums) {
                 const float4 s = table[j * 8 + 1];
-                total[0][0] = __fmaf_rn(c[0][1], s.z, __fmaf_rn(c[0][0], s.x, total[0][0]));
-                total[0][1] = __fmaf_rn(c[0][1], s.w, __fmaf_rn(c[0][0], s.y, total[0][1]));
-                total[0][2] = __fmaf_rn(c[1][1], s.z, __fmaf_rn(c[1][0], s.x, total[0][2]));
-                total[0][3] = __fmaf_rn(c[1][1], s.w, __fmaf_rn(c[1][0], s.y, total[0][3]));
+                add_scaled(total[0], c[0][0], c[1][0], s.x, s.y, s.x, s.y);
+                add_scaled(total[0], c[0][1], c[1][1], s.z, s.w, s.z, s.w);
             }
             ahead.fetch_quads(b, j);
         }
