@@ -65,6 +65,9 @@ class Status(enum.IntEnum):
     OUT_OF_MEMORY = 19
 
 
+_STATUSES = {int(s): s for s in Status}  # quicker than the enum's call
+
+
 class BinaryOp(enum.IntEnum):
     ADD = 0
     SUB = 1
@@ -256,13 +259,14 @@ SIGNATURES = {
     "emel_cuda_cpy": (_I, [_CTX, _V, _P, _P]),
     "emel_cuda_cont": (_I, [_CTX, _V, _P, _P]),
     "emel_cuda_glu": (_I, [_CTX, _V, _I, _V, ctypes.c_uint64, _V, ctypes.c_uint64]),
-    "emel_cuda_paged_kv_append": (_I, [_CTX, _V, _P, _P, _P, _P, _P, _P, _P]),
-    "emel_cuda_paged_attn": (_I, [_CTX, _V, _P, _P, _P, _P, _P, _P, ctypes.POINTER(CPagedAttnOptions)]),
+    # the decoding-step events pass the addresses of views that they hold
+    "emel_cuda_paged_kv_append": (_I, [_CTX, _V, _V, _V, _V, _V, _V, _V, _V]),
+    "emel_cuda_paged_attn": (_I, [_CTX, _V, _V, _V, _V, _V, _V, _V, _V]),
     "emel_cuda_q4_packed_bytes": (_I, [ctypes.c_uint32, ctypes.c_uint64, ctypes.c_uint64,
                                        ctypes.POINTER(ctypes.c_uint64)]),
     "emel_cuda_q4_pack": (_I, [_CTX, _V, _P, _V, ctypes.c_uint64, ctypes.POINTER(CQ4Weights)]),
-    "emel_cuda_mul_mat_q4": (_I, [_CTX, _V, ctypes.POINTER(CQ4Weights), _P, _P]),
-    "emel_cuda_logits_adjust": (_I, [_CTX, _V, _P, _P, _P, _P, _P, _P, _P]),
+    "emel_cuda_mul_mat_q4": (_I, [_CTX, _V, _V, _V, _V]),
+    "emel_cuda_logits_adjust": (_I, [_CTX, _V, _V, _V, _V, _V, _V, _V, _V]),
     "emel_cuda_exchange_create": (_I, [_CTX, _I, _I, ctypes.c_uint32, ctypes.c_uint32, ctypes.POINTER(_V)]),
     "emel_cuda_exchange_handle": (_I, [_V, _V]),
     "emel_cuda_exchange_connect": (_I, [_CTX, _V, _V]),
@@ -1069,8 +1073,28 @@ class OpGlu(Event):
 # One decoding step: paged cache, its attention, 4-bit projections, logits
 # ---------------------------------------------------------------------------
 
-@dataclass
-class OpPagedKvAppend(Event):
+class _StepEvent(Event):
+    """An event of a decoding step, built once and dispatched every step: its
+    fields are fixed, and where all its views are CViews their addresses are kept,
+    so that a dispatch is one foreign call (what a CView holds may change)."""
+    VIEWS = ()
+
+    def __post_init__(self):
+        views = [getattr(self, name) for name in self.VIEWS]
+        for v in views:
+            if v is not None and not isinstance(v, (CView, TensorView)):
+                raise TypeError(f"{type(self).__name__} takes views, not {type(v).__name__}")
+        fixed = all(v is None or isinstance(v, CView) for v in views)
+        object.__setattr__(self, "_at", tuple(v and ctypes.addressof(v) for v in views) if fixed else None)
+
+    def _args(self):
+        if self._at is not None:
+            return self._at
+        return tuple(_r(getattr(self, name)) for name in self.VIEWS)
+
+
+@dataclass(frozen=True)
+class OpPagedKvAppend(_StepEvent):
     """New keys and values [d, kv_heads, count] into the pages of a cache
     [d, kv_heads, page_size, pages] (emel_cuda_paged_kv_append): row i goes to
     position positions[i] of sequence sequences[i] (None: of sequence i)."""
@@ -1081,15 +1105,14 @@ class OpPagedKvAppend(Event):
     positions: TensorView
     key_cache: TensorView
     value_cache: TensorView
+    VIEWS = ("key", "value", "block_table", "sequences", "positions", "key_cache", "value_cache")
 
     def dispatch(self, ctx, stream):
-        return ctx._lib.emel_cuda_paged_kv_append(ctx.handle, stream, _r(self.key), _r(self.value),
-                                                  _r(self.block_table), _r(self.sequences), _r(self.positions),
-                                                  _r(self.key_cache), _r(self.value_cache))
+        return ctx._lib.emel_cuda_paged_kv_append(ctx.handle, stream, *self._args())
 
 
-@dataclass
-class OpPagedAttn(Event):
+@dataclass(frozen=True)
+class OpPagedAttn(_StepEvent):
     """One new token of every sequence, query / destination [d, heads, batch],
     over its cached tokens (emel_cuda_paged_attn).  scale: None for
     1 / sqrt(d); window: how many of the last tokens are seen, 0 for all."""
@@ -1101,12 +1124,15 @@ class OpPagedAttn(Event):
     destination: TensorView
     scale: Optional[float] = None
     window: int = 0
+    VIEWS = ("query", "key_cache", "value_cache", "block_table", "lengths", "destination")
+
+    def __post_init__(self):
+        super().__post_init__()
+        opts = CPagedAttnOptions(self.scale or 0.0, self.scale is not None, self.window, 0)
+        object.__setattr__(self, "_options", (opts, ctypes.addressof(opts)))
 
     def dispatch(self, ctx, stream):
-        opts = CPagedAttnOptions(self.scale or 0.0, self.scale is not None, self.window, 0)
-        return ctx._lib.emel_cuda_paged_attn(ctx.handle, stream, _r(self.query), _r(self.key_cache),
-                                             _r(self.value_cache), _r(self.block_table), _r(self.lengths),
-                                             _r(self.destination), ctypes.byref(opts))
+        return ctx._lib.emel_cuda_paged_attn(ctx.handle, stream, *self._args(), self._options[1])
 
 
 class Q4Weights:
@@ -1122,6 +1148,7 @@ class Q4Weights:
                "q4_packed_bytes")
         self.buffer = DeviceBuffer(ctx, need.value)
         self.c = CQ4Weights()
+        self.at = ctypes.addressof(self.c)
         _check(ctx._lib.emel_cuda_q4_pack(ctx.handle, stream, ctypes.byref(view), ctypes.c_void_p(self.buffer.ptr),
                                           need.value, ctypes.byref(self.c)), "q4_pack")
 
@@ -1129,21 +1156,21 @@ class Q4Weights:
         self.buffer.free()
 
 
-@dataclass
-class OpMulMatQ4(Event):
+@dataclass(frozen=True)
+class OpMulMatQ4(_StepEvent):
     """destination [rows, n] = weights [k, rows] times rhs [k, n], for one or a
     few columns n (emel_cuda_mul_mat_q4)."""
     weights: Q4Weights
     rhs: TensorView
     destination: TensorView
+    VIEWS = ("rhs", "destination")
 
     def dispatch(self, ctx, stream):
-        return ctx._lib.emel_cuda_mul_mat_q4(ctx.handle, stream, ctypes.byref(self.weights.c), _r(self.rhs),
-                                             _r(self.destination))
+        return ctx._lib.emel_cuda_mul_mat_q4(ctx.handle, stream, self.weights.at, *self._args())
 
 
-@dataclass
-class OpLogitsAdjust(Event):
+@dataclass(frozen=True)
+class OpLogitsAdjust(_StepEvent):
     """Penalties for repeated tokens, biases and the mask of allowed tokens on
     logits [vocab, rows] (emel_cuda_logits_adjust).  history, history_lengths
     and penalties (repetition, frequency, presence) come together or not at
@@ -1155,11 +1182,10 @@ class OpLogitsAdjust(Event):
     penalties: Optional[TensorView] = None
     bias: Optional[TensorView] = None
     allowed: Optional[TensorView] = None
+    VIEWS = ("src", "history", "history_lengths", "penalties", "bias", "allowed", "dst")
 
     def dispatch(self, ctx, stream):
-        return ctx._lib.emel_cuda_logits_adjust(ctx.handle, stream, _r(self.src), _r(self.history),
-                                                _r(self.history_lengths), _r(self.penalties), _r(self.bias),
-                                                _r(self.allowed), _r(self.dst))
+        return ctx._lib.emel_cuda_logits_adjust(ctx.handle, stream, *self._args())
 
 
 class Kernel:
@@ -1175,8 +1201,8 @@ class Kernel:
         self.synchronize = synchronize
 
     def process_event(self, event: Event) -> Status:
-        st = Status(event.dispatch(self.ctx, self.stream))
-        if st == Status.OK and self.synchronize:
+        st = _STATUSES[event.dispatch(self.ctx, self.stream)]
+        if self.synchronize and st is Status.OK:
             self.ctx.synchronize(self.stream)
         return st
 
