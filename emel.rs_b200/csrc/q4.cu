@@ -417,23 +417,25 @@ __device__ __forceinline__ void load_piece(const Q4MatvecPlan& p, bool vec, uint
     if constexpr (F32) v[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-// The largest finite magnitude (bits) among eight binary32 values.
+// The largest magnitude (bits) among eight binary32 values: above kInfinity if
+// one is a NaN.
+constexpr uint32_t kInfinity = 0x7f800000u;
 __device__ __forceinline__ uint32_t largest_of(const uint32_t (&w)[8]) {
     uint32_t big = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint32_t b = w[e] & 0x7fffffffu;
-        big = b < 0x7f800000u && b > big ? b : big;
-    }
+    for (int e = 0; e < 8; ++e) big = max(big, w[e] & 0x7fffffffu);
     return big;
 }
 
-// The power of two that brings `largest` (bits) into [2^to, 2^(to + 1)), as far
-// as it is a normal number.
-__device__ __forceinline__ float scale_to(uint32_t largest, int to) {
+// The exponent field of the power of two that brings `largest` (bits, finite)
+// into [2^to, 2^(to + 1)), as far as it is a normal number; of 1 for 0.
+__device__ __forceinline__ uint32_t scale_to(uint32_t largest, int to) {
     const int e = 127 + to + 127 - (int)(largest >> 23);
-    return largest == 0 ? 1.0f : bitsf((uint32_t)(e > 254 ? 254 : e) << 23);
+    return largest == 0 ? 127u : (uint32_t)(e > 254 ? 254 : e);
 }
+__device__ __forceinline__ float power(uint32_t field) { return bitsf(field << 23); }
+// 1 / power(field), a subnormal for the largest
+__device__ __forceinline__ float inverse_power(uint32_t field) { return bitsf(field < 254 ? (254 - field) << 23 : 0x00400000u); }
 
 // The sums of a round: every warp's [16 rows][COLS] lie in shared memory, 8
 // floats apart beyond their size; the output (tile, row, token) is the sum over
@@ -625,13 +627,32 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_halves_kernel(const Q4Mat
     }
     __syncthreads();
     if (PARTS == 2) {
+        uint32_t special = 0;  // tokens with an infinity or a NaN: their largest finite value is found anew
+        for (uint32_t i = 0; i < n; ++i) special |= (uint32_t)(sh.top[i] >= kInfinity) << i;
+        if (special) {
+            __syncthreads();
+            if (threadIdx.x < n && ((special >> threadIdx.x) & 1u)) sh.top[threadIdx.x] = 0;
+            __syncthreads();
+            if (threadIdx.x < all) {
+                Q4Piece x{threadIdx.x / pieces, threadIdx.x % pieces};
+                for (uint32_t i = threadIdx.x; i < all; i += kQ4MulThreads, x.next(pieces)) {
+                    if (!((special >> x.token) & 1u)) continue;
+                    const uint4 a = *hi_slot(x), b = *lo_slot(x);
+                    const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    for (int e = 0; e < 8; ++e)
+                        if ((v[e] & 0x7fffffffu) < kInfinity) atomicMax(sh.top + x.token, v[e] & 0x7fffffffu);
+                }
+            }
+            __syncthreads();
+        }
         if (threadIdx.x < all) {
             Q4Piece x{threadIdx.x / pieces, threadIdx.x % pieces};
             for (uint32_t i = threadIdx.x; i < all; i += kQ4MulThreads) {
                 const uint4 a = *hi_slot(x), b = *lo_slot(x);
                 const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                const float scale = scale_to(sh.top[x.token], 14);
-                if (x.at == 0) sh.up[x.token] = 1.0f / scale;
+                const uint32_t field = scale_to(sh.top[x.token], 14);
+                const float scale = power(field);
+                if (x.at == 0) sh.up[x.token] = inverse_power(field);
                 float sum = 0.0f;
                 uint32_t hi[4], lo[4];
 #pragma unroll
@@ -639,9 +660,13 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_halves_kernel(const Q4Mat
                     const float y = bitsf(v[2 * q]) * scale, z = bitsf(v[2 * q + 1]) * scale;
                     const __half2 h = __floats2half2_rn(y, z);
                     const float2 f = __half22float2(h);
-                    const float ry = y - f.x, rz = z - f.y;  // NaN for an infinity: the first part carries it alone
+                    float ry = y - f.x, rz = z - f.y;
+                    if (special) {  // NaN for an infinity: the first part carries it alone
+                        ry = fabsf(ry) < INFINITY ? ry : 0.0f;
+                        rz = fabsf(rz) < INFINITY ? rz : 0.0f;
+                    }
                     hi[q] = h2_bits(h);
-                    lo[q] = h2_bits(__floats2half2_rn(fabsf(ry) < INFINITY ? ry : 0.0f, fabsf(rz) < INFINITY ? rz : 0.0f));
+                    lo[q] = h2_bits(__floats2half2_rn(ry, rz));
                     sum += y + z;
                 }
                 *hi_slot(x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -786,18 +811,18 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4Mat
                 y[2 * e] = bitsf(b.x);
                 y[2 * e + 1] = bitsf(b.y);
             }
-            const float scale = scale_to(sh.top[x.token], 29);
-            bool lost = false;  // an infinity or NaN: it takes the whole column
+            const uint32_t largest = sh.top[x.token], field = largest >= kInfinity ? 127u : scale_to(largest, 29);
+            const float scale = power(field);
             uint32_t d[8];
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                lost = lost || !(fabsf(y[e]) < INFINITY);
                 const int X = __float2int_rn(y[e] * scale);
                 if constexpr (kSums) sum += (float)X;
                 d[e] = ((uint32_t)X + 0x00808080u) ^ 0x00808080u;  // four balanced digits
             }
-            if (x.at == 0) sh.up[x.token] = 1.0f / scale;
+            // an infinity or NaN takes the whole column
+            if (x.at == 0) sh.up[x.token] = largest >= kInfinity ? bitsf(0x7fc00000u) : inverse_power(field);
             // bytes i of the columns 0, 2, 1, 3 and 4, 6, 5, 7
             uint32_t digit[4][2];
 #pragma unroll
@@ -826,12 +851,10 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4Mat
                     if constexpr (kSums) (&e)[4] = q == 3 ? sum * (1.0f / 16777216.0f) : 0.0f;
                 }
             }
-            if (__any_sync(0xffffffffu, lost) && w.lane == 0) sh.top[x.token] = 0xffffffffu;
             x.next(pieces);
         }
     }
     __syncthreads();
-    if (threadIdx.x < n && sh.top[threadIdx.x] == 0xffffffffu) sh.up[threadIdx.x] = bitsf(0x7fc00000u);
 
     const uint32_t g = w.lane >> 2, t = w.lane & 3u;
     // lanes of unused columns read the first one: their results are not used

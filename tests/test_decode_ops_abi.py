@@ -76,6 +76,18 @@ def test_attention(emel):
     assert attn(emel, opts=emel.CPagedAttnOptions(0.0, 0, 7, 1)) == PARAMS
 
 
+def test_events_take_views_and_keep_their_fields(emel):
+    v = view(emel, 0, (64, 8, 3), "f32")
+    with pytest.raises(TypeError):
+        emel.OpLogitsAdjust(v, 7)
+    event = emel.OpLogitsAdjust(v, v)
+    with pytest.raises(Exception):
+        event.src = v
+    assert event.dispatch(type("Ctx", (), {"_lib": emel.lib(), "handle": None}), None) == SHAPE
+    v.ne[2] = 1  # what a view holds may change
+    assert event.dispatch(type("Ctx", (), {"_lib": emel.lib(), "handle": None}), None) == OK
+
+
 def append(emel, **change):
     a = {"key": ((64, 2, 7), "f32"), "value": ((64, 2, 7), "f32"), "table": ((5, 3), "i32"), "seq": ((7,), "i32"),
          "pos": ((7,), "i32"), "k": ((64, 2, 16, 10), "f16"), "v": ((64, 2, 16, 10), "f16")}
@@ -158,6 +170,7 @@ def test_product(emel):
     assert call(y=((20, 3), "f32", {"nb": [8, 160, 480, 480]})) == LAYOUT
     assert call(x=((256, 3), "f32")) == SHAPE and call(x=((512, 4), "f32")) == SHAPE and call(y=((21, 3), "f32")) == SHAPE
     assert call(x=((512, 3, 2), "f32")) == SHAPE
+    assert call(k=131072) == OK and call(k=131072 + 32) == SHAPE
     assert lib.emel_cuda_mul_mat_q4(None, None, None, None, None) == VIEW
 
 

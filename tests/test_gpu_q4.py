@@ -128,6 +128,34 @@ def test_not_finite_activations_stay_in_their_column(emel, kern):
     assert top.sum() >= 20
 
 
+@pytest.mark.parametrize("x", ["f32", "f16"])
+def test_not_finite_activations_of_one_or_two_tokens(emel, kern, x):
+    rng = np.random.default_rng(4)
+    raw = dh.q4_random(rng, "q4_0", 40, 512)
+    blocks = Blocks(emel, kern.ctx, raw, "q4_0")
+    w = emel.Q4Weights(kern.ctx, blocks.c())
+    for bad in (np.nan, np.inf, -np.inf):
+        act = rng.standard_normal((2, 512)).astype(np.float32)
+        act[0, 333] = bad
+        xd, yd = dh.Dev(emel, kern.ctx, act, x), dh.Dev(emel, kern.ctx, np.zeros((2, 40)), "f32")
+        assert kern.process_event(emel.OpMulMatQ4(w, xd.c(), yd.c())) == 0
+        got = yd.read()
+        assert not np.isfinite(got[0]).any()
+        tol = (64 + 16) * 2.0 ** -23 * (np.abs(xd.values[1]) @ parts(raw, "q4_0").T)
+        assert (np.abs(got[1] - xd.values[1] @ dh.q4_values(raw, "q4_0").T) <= tol).all()
+
+
+def test_columns_of_zeros(emel, kern):
+    rng = np.random.default_rng(14)
+    raw = dh.q4_random(rng, "q4_1", 33, 320)
+    blocks = Blocks(emel, kern.ctx, raw, "q4_1")
+    w = emel.Q4Weights(kern.ctx, blocks.c())
+    for n in (1, 2, 3, 8):
+        xd, yd = dh.Dev(emel, kern.ctx, np.zeros((n, 320)), "f32"), dh.Dev(emel, kern.ctx, np.full((n, 33), 5.0), "f32")
+        assert kern.process_event(emel.OpMulMatQ4(w, xd.c(), yd.c())) == 0
+        assert (yd.read() == 0).all()
+
+
 def test_the_same_call_gives_the_same_bits_on_another_stream(emel, kern):
     rng = np.random.default_rng(5)
     ctx = kern.ctx
