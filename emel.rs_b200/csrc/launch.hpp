@@ -247,7 +247,6 @@ struct PagedAttnPlan {
     int64_t len_st;
     uint64_t d, heads, batch, rep, page_size, pages;
     uint64_t window;        // 0: every cached token is seen
-    uint64_t min_run;       // set by the launcher: tiles of a CTA at least
     uint64_t page_mul;      // set by the launcher: t / page_size = (t * page_mul) >> page_shift
     uint32_t page_shift;
     float scale;

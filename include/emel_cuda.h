@@ -833,11 +833,12 @@ EMEL_CUDA_API emel_cuda_status emel_cuda_q4_pack(emel_cuda_context* ctx, void* s
                                                  void* data, uint64_t bytes, emel_q4_weights* out);
 /* dst[r, i] = sum over c of w[r, c] * rhs[c, i]: rhs [k, n] F32 or F16, dst
  * [rows, n] F32 or F16, unit rows.  Weights count with their exact values
- * (d (q - 8), d q + m, d s q - e t), products are exact and sums binary32,
- * rounded once to dst's type.  A matrix-vector product for single tokens and
+ * (d (q - 8), d q + m, d s q - e t), products of a group of 32 are summed before
+ * they meet its scale, sums are binary32, rounded once to dst's type.  A matrix-vector product for single tokens and
  * small batches: every further 8 columns of rhs read the weights once more.
- * Weights' scales must be finite.  An F32 activation counts with 22 bits or
- * more of its value, down to 2^-40 of its column's largest finite one.
+ * Weights' scales must be finite.  An activation counts to within 2^-23 of its
+ * own value or 2^-30 of its column's largest finite one, whichever is more; a
+ * column with an infinity or a NaN gives what is not finite.
  * Statuses: INVALID_VIEW (views or weights), INVALID_LAYOUT, SHAPE_MISMATCH
  * (k > 131072 among them),
  * INVALID_ARGUMENT (null context, dst overlapping rhs or the weights). */
