@@ -1899,6 +1899,7 @@ emel_cuda_status emel_cuda_q4_pack(emel_cuda_context* ctx, void* stream, const e
     p.rows = src->ne[1];
     p.row_bytes = row_bytes;
     p.code = (int)src->dtype;
+    p.even = reinterpret_cast<uintptr_t>(src->data) % 2 == 0;
     cudaError_t err = select_device(ctx);
     if (err == cudaSuccess) err = emel::launch_q4_pack(env_of(ctx, stream), p);
     if (err == cudaSuccess) *out = emel_q4_weights{data, need, p.k, p.rows, src->dtype, 0};

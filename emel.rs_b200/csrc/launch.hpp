@@ -274,6 +274,7 @@ struct Q4PackPlan {
     uint8_t* dst;           // packed layout, 16-byte aligned
     uint64_t k, rows, row_bytes;
     int code;
+    bool even;              // src on a 2-byte boundary: so is every block
 };
 
 struct Q4MatvecPlan {

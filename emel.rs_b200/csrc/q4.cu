@@ -38,19 +38,26 @@ __host__ __device__ constexpr uint64_t q4_scale_bytes(int code) {
     return code == kDtypeQ4_0 ? 256 : code == kDtypeQ4_1 ? 512 : 320;
 }
 
-// The quant of column k in a source row.
+// Quants k .. k + 3 of a source row (k a multiple of 4), one in the low half of
+// each byte: adjacent columns stand in adjacent bytes, of one half or the other.
 template <int CODE>
-__device__ __forceinline__ uint32_t q4_quant(const uint8_t* row, uint64_t k) {
+__device__ __forceinline__ uint32_t q4_quants(const uint8_t* row, uint64_t k, bool even) {
     const uint32_t i = (uint32_t)k & 31u;
+    const uint8_t* from;
+    bool high;
     if constexpr (CODE == kDtypeQ4_K) {
         const uint32_t sub = ((uint32_t)k & 255u) >> 5;
-        const uint8_t byte = row[(k >> 8) * 144 + 16 + 32 * (sub >> 1) + i];
-        return (sub & 1u) ? byte >> 4 : byte & 15u;
+        from = row + (k >> 8) * 144 + 16 + 32 * (sub >> 1) + i;
+        high = sub & 1u;
     } else {
         constexpr int kBlock = CODE == kDtypeQ4_0 ? 18 : 20;
-        const uint8_t byte = row[(k >> 5) * kBlock + (kBlock - 16) + (i & 15u)];
-        return i < 16 ? byte & 15u : byte >> 4;
+        from = row + (k >> 5) * kBlock + (kBlock - 16) + (i & 15u);
+        high = i >= 16;
     }
+    uint32_t v;
+    if (even) v = reinterpret_cast<const uint16_t*>(from)[0] | (uint32_t)reinterpret_cast<const uint16_t*>(from)[1] << 16;
+    else v = from[0] | (uint32_t)from[1] << 8 | (uint32_t)from[2] << 16 | (uint32_t)from[3] << 24;
+    return (high ? v >> 4 : v) & 0x0f0f0f0fu;
 }
 
 __device__ __forceinline__ uint32_t load16(const uint8_t* p) { return (uint32_t)p[0] | ((uint32_t)p[1] << 8); }
@@ -76,13 +83,10 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackPlan p) {
                 const uint64_t k = kb * 64 + 32 * (j >> 1) + 8 * t + 4 * (j & 1);
                 w[j] = 0;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint64_t kk = k + 2 * (r >> 1) + h, rr = row[r & 1];
-                        const uint32_t q = rr < p.rows && kk < p.k ? q4_quant<CODE>(p.src + rr * p.row_bytes, kk) : 8u;
-                        w[j] |= q << (4 * r + 16 * h);
-                    }
+                for (int h = 0; h < 2; ++h) {  // rows g and g + 8: columns k, k + 2, k + 1, k + 3 in a word's bytes
+                    const uint32_t q = row[h] < p.rows && k < p.k ? q4_quants<CODE>(p.src + row[h] * p.row_bytes, k, p.even) : 0x08080808u;
+                    w[j] |= __byte_perm(q, 0, 0x3120) << (4 * h);
+                }
             }
             reinterpret_cast<uint4*>(p.dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
             continue;
