@@ -11,7 +11,7 @@
 // counts the ids that fall into its tokens in shared memory (integer atomics: the
 // counts do not depend on their order); a row is read once from HBM, its
 // history once per chunk from L2.  64 rows of 151936 logits with biases and masks
-// for each row: 18.9 us without a history (18.0 at the copy rate), 26.1 us with up to
+// for each row: 18.9 us without a history (18.0 at the copy rate), 25.9 us with up to
 // 4096 ids a row.  Chunks of 8192 took 33 us, chunks of 2048 42 us (more waves of
 // history), and anything that spills registers a third more.
 #include <cuda_fp16.h>
