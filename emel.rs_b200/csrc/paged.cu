@@ -163,8 +163,8 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan 
 // knows them.
 //
 // Bound by HBM once the lengths, the table and the rows have come one after another.
-// 32 heads over 8 of 128: 64 sequences of up to 8191 tokens in bfloat16, 673 MB, 121 us,
-// 5.6 TB/s; one of 32768 tokens, binary32 over binary16, 134 MB, 34.5 us, 3.9 TB/s
+// 32 heads over 8 of 128: 64 sequences of up to 8191 tokens in bfloat16, 673 MB, 124 us,
+// 5.4 TB/s; one of 32768 tokens, binary32 over binary16, 134 MB, 34.5 us, 3.9 TB/s
 // (start and joins are latency).
 //
 // Tile.  Four warps take 16 of a tile's tokens each; two more find the rows
@@ -180,7 +180,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan 
 //
 // Products on m16n8k16: S[head, token] = Q K^T, whose result fragments are
 // the operand fragments of O[head, d] += P V.  Sixteen heads of a 16-bit
-// query fill the 16 rows.  A binary32 query keeps its precision by parts
+// query fill the 16 rows; their weights meet the values in two 16-bit parts (22 bits in
+// binary16, 17 in bfloat16: the result is rounded to 11 or 8), one operand after the
+// other.  A binary32 query keeps its precision by parts
 // instead: 8 heads, rows 0..7 the parts of highest weight, rows 8..15 the
 // next ones -- binary16 caches: 2 parts of 11 bits, of the query divided by
 // the power of two that brings its largest element into [1, 2), and of the
@@ -677,12 +679,16 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                     o[n][3] *= keep[kHeadsLane - 1];
                 }
             }
-            uint32_t a0, a1, a2, a3, c0 = 0, c2 = 0;
+            uint32_t a0, a1, a2, a3, c0 = 0, c1 = 0, c2 = 0, c3 = 0;
             a0 = pack2<C>(w[0][0], w[0][1]);
             a2 = pack2<C>(w[0][2], w[0][3]);
             if constexpr (PARTS == 1) {
                 a1 = pack2<C>(w[1][0], w[1][1]);
                 a3 = pack2<C>(w[1][2], w[1][3]);
+                c0 = pack2<C>(rest_of<C>(w[0][0]), rest_of<C>(w[0][1]));
+                c2 = pack2<C>(rest_of<C>(w[0][2]), rest_of<C>(w[0][3]));
+                c1 = pack2<C>(rest_of<C>(w[1][0]), rest_of<C>(w[1][1]));
+                c3 = pack2<C>(rest_of<C>(w[1][2]), rest_of<C>(w[1][3]));
             } else {
                 float r[4];
 #pragma unroll
@@ -700,9 +706,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
                 ldsm4_t(b, base + v_at + n * 32);
                 mma16816<C>(o[2 * n], a0, a1, a2, a3, b[0], b[1]);
                 mma16816<C>(o[2 * n + 1], a0, a1, a2, a3, b[2], b[3]);
-                if constexpr (PARTS == 3) {
-                    mma16816<C>(o[2 * n], c0, 0u, c2, 0u, b[0], b[1]);
-                    mma16816<C>(o[2 * n + 1], c0, 0u, c2, 0u, b[2], b[3]);
+                if constexpr (PARTS != 2) {
+                    mma16816<C>(o[2 * n], c0, c1, c2, c3, b[0], b[1]);
+                    mma16816<C>(o[2 * n + 1], c0, c1, c2, c3, b[2], b[3]);
                 }
             }
         }

@@ -788,8 +788,9 @@ EMEL_CUDA_API emel_cuda_status emel_cuda_paged_kv_append(emel_cuda_context* ctx,
  * score is -inf; a NaN or +inf score, or a value that is not finite, gives
  * what is not finite.  Whatever lies in the cache beyond the n tokens (or before
  * the window) has no effect, NaN and infinities included.  Scores, weights'
- * sums and products are binary32; 16-bit queries round the weights to the
- * cache's type before they meet the values.  A length beyond the table
+ * sums and products are binary32, rounded once to dst's type; a weight counts
+ * to within 2^-21 of its own value (16-bit queries over BF16: 2^-17) or 2^-32 of
+ * the largest one's, whichever is more.  A length beyond the table
  * is taken as the table's and rejected (see above); tokens of a rejected page
  * are left out.  dst may not overlap an input.
  * options NULL: scale 1 / sqrt(d), no window.

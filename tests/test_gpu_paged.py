@@ -172,6 +172,25 @@ def test_infinite_scores(emel, kern):
     assert np.isnan(got[2]).all()
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("kvh,rep,d", [(2, 1, 8), (1, 4, 16), (1, 9, 8), (1, 17, 16)])
+def test_16_bit_queries_round_only_the_result(emel, kern, kind, kvh, rep, d):
+    """Before its rounding the result is within the binary32 bar (a score moves by (d + 16) 2^-23 S, sums over n
+    tokens by (n + 16) 2^-23) and 2^-17 for weights in two parts: no room for 16-bit weights.  Rounding is
+    monotone, so the result lies between the rounded ends."""
+    q, k, v, table, lengths, out = setup(emel, kern.ctx, rep, [16] * 40 + [5, 30], kvh, rep, d, 7, kind, kind)
+    assert kern.process_event(emel.OpPagedAttn(q.c(), k.c(), v.c(), table.c(), lengths.c(), out.c())) == 0
+    got = out.read()
+    want = dh.attention(q.values, k.values, v.values, table.values, lengths.values, 1 / np.sqrt(d))
+    for b, n in enumerate(lengths.values):
+        where = table.values[b, np.arange(n) // 7], np.arange(n) % 7
+        for h in range(kvh * rep):
+            s = (np.abs(k.values[where][:, h // rep]) @ np.abs(q.values[b, h])).max() / np.sqrt(d)
+            tol = np.abs(v.values[where][:, h // rep]).max() * (2 * (d + 16) * 2.0 ** -23 * s + (n + 16) * 2.0 ** -23 + 2.0 ** -17)
+            lo, hi = (dh.store(want[b, h] + e, kind)[1] for e in (-tol, tol))
+            assert ((lo <= got[b, h]) & (got[b, h] <= hi)).all(), (b, h)
+
+
 def test_padding_of_the_destination_is_not_written(emel, kern):
     devs = setup(emel, kern.ctx, 12, [40, 3], 2, 2, 40, 16, pad=5, skip=3)
     check(emel, kern, devs)
