@@ -301,7 +301,9 @@ __device__ __forceinline__ int64_t divided(int64_t a, int64_t b) {
     return ((uint64_t)(a | b) >> 32) == 0 ? (int64_t)((uint32_t)a / (uint32_t)b) : a / b;
 }
 
-// A token's row: its page (-2: no token, -1: not known) and place in it.
+// A token's row: its page as the table has it, whatever that is, and place in it
+// (kNoToken: there is no token; a page has less than 2^31 places).
+constexpr uint32_t kNoToken = 0xffffffffu;
 struct RowAt {
     int32_t page;
     uint32_t off;
@@ -434,14 +436,14 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
 
     auto row_of = [&](const TileAt& x, uint32_t token) -> RowAt {
         const uint32_t t = (uint32_t)x.first + x.tile * kAttnTile + token;  // at most 63 beyond a length
-        if (t >= (uint32_t)x.len) return RowAt{-2, 0};
+        if (t >= (uint32_t)x.len) return RowAt{-1, kNoToken};
         // t / page_size by the host's multiplier (t < 2^31)
         const uint32_t at = (uint32_t)(((uint64_t)t * p.page_mul) >> p.page_shift);
         return RowAt{p.table[(int64_t)at * p.table_st[0] + (int64_t)x.b * p.table_st[1]], t - at * page_size};
     };
     auto known = [&](const RowAt& r) {
         const bool in = (uint64_t)(int64_t)r.page < p.pages;  // a negative page is a huge number
-        if (!in && r.page != -2) atomicExch(p.reject, p.reject_code);
+        if (!in && r.off != kNoToken) atomicExch(p.reject, p.reject_code);
         return in;
     };
     auto key_row = [&](const TileAt& x, const RowAt& r) {

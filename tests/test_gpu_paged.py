@@ -222,6 +222,18 @@ def test_pages_outside_the_cache_are_rejected(emel, kern):
     check(emel, kern, (q, k, v, table, lengths, out))  # nothing of the rejected call is left
 
 
+@pytest.mark.parametrize("page", [-1, -2, -3, 1 << 20, 2 ** 31 - 1, -2 ** 31])
+@pytest.mark.parametrize("pad", [0, 1])
+def test_every_page_number_outside_the_cache_is_reported(emel, kern, page, pad):
+    q, k, v, table, lengths, out = setup(emel, kern.ctx, 13, [100, 50], 1, 2, 64, 16, pad=pad)
+    t = table.values.copy()
+    t[0, 2] = page
+    bad = dh.Dev(emel, kern.ctx, t, "i32")
+    quiet = emel.Kernel(ctx=kern.ctx)
+    assert quiet.process_event(emel.OpPagedAttn(q.c(), k.c(), v.c(), bad.c(), lengths.c(), out.c())) == 0
+    assert kern.ctx._lib.emel_cuda_stream_synchronize(kern.ctx.handle, None) == 9
+
+
 def test_lengths_outside_the_table_are_rejected(emel, kern):
     q, k, v, table, lengths, out = setup(emel, kern.ctx, 14, [32, 20], 1, 2, 64, 16)
     far = dh.Dev(emel, kern.ctx, [33, -5], "i32")
