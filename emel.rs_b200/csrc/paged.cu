@@ -379,8 +379,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
     }
     if (blockIdx.x == 0) {
         for (int32_t b = threadIdx.x; b < batch; b += kAttnThreads) {
-            const int32_t raw = p.lengths[b * p.len_st];
-            bad = bad || raw < 0 || raw > cap;
+            bad = bad || p.lengths[b * p.len_st] > cap;  // a negative length is an empty sequence
         }
         if (bad) atomicExch(p.reject, p.reject_code);
     }

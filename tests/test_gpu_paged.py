@@ -245,6 +245,15 @@ def test_lengths_outside_the_table_are_rejected(emel, kern):
     assert np.abs(got - want).max() < 1e-5
 
 
+def test_negative_lengths_are_empty_sequences(emel, kern):
+    """They give zeros and nothing to report: a padded row of a captured step beside the append's negative position."""
+    q, k, v, table, lengths, out = setup(emel, kern.ctx, 14, [32, 20, 7], 1, 2, 64, 16)
+    below = dh.Dev(emel, kern.ctx, [32, -5, -2 ** 31], "i32")
+    check(emel, kern, (q, k, v, table, below, out))
+    assert kern.ctx._lib.emel_cuda_stream_synchronize(kern.ctx.handle, None) == 0
+    assert (out.read()[1:] == 0).all()
+
+
 def test_replay_reads_new_lengths_and_the_same_inputs_give_the_same_bits(emel, kern):
     ctx = kern.ctx
     stream = emel.Stream(ctx)
