@@ -436,12 +436,14 @@ __device__ __forceinline__ uint32_t largest_of(const uint32_t (&w)[8]) {
     return big;
 }
 
-// The exponent field of the power of two that brings `largest` (bits, finite)
-// into [2^to, 2^(to + 1)), as far as it is a normal number; of 1 for 0.
+// The exponent field (127 + e) of the power of two 2^e that brings `largest` (bits,
+// finite) into [2^to, 2^(to + 1)), or below where it is subnormal; of 1 for 0.  Above
+// 254 it is no number's: e is then 127 and a rest, two exact steps.
 __device__ __forceinline__ uint32_t scale_to(uint32_t largest, int to) {
-    const int e = 127 + to + 127 - (int)(largest >> 23);
-    return largest == 0 ? 127u : (uint32_t)(e > 254 ? 254 : e);
+    return largest == 0 ? 127u : (uint32_t)(127 + to + 127 - (int)(largest >> 23));
 }
+__device__ __forceinline__ uint32_t first_step(uint32_t field) { return field > 254 ? 254u : field; }
+__device__ __forceinline__ uint32_t rest_step(uint32_t field) { return 127 + field - first_step(field); }
 __device__ __forceinline__ float power(uint32_t field) { return bitsf(field << 23); }
 // 1 / power(field), a subnormal for the largest
 __device__ __forceinline__ float inverse_power(uint32_t field) { return bitsf(field < 254 ? (254 - field) << 23 : 0x00400000u); }
@@ -481,6 +483,7 @@ __device__ __forceinline__ void q4_join(const Q4MatvecPlan& p, const Q4Shape& sh
         all += __shfl_xor_sync(0xffffffffu, all, 8);
         all += __shfl_xor_sync(0xffffffffu, all, 16);
         if (quarter == 0) {
+            if constexpr (PARTS == 4) all *= up[kQ4Tokens + token];  // digits: exact, the last rounding is the next one
             all *= up[token];
             if (shape.splits > 1) part[(round & 1u) * outs + o] = all;
             else store(row, token, all);
@@ -543,7 +546,7 @@ template <int NT>
 struct Q4Shared {
     float* red;      // [2][warp][16][8 NT], padded
     float* part;     // [2][wr * 16 * n], splits > 1
-    float* up;       // [kQ4Tokens]: 2^-e
+    float* up;       // [2][kQ4Tokens]: 2^-e of the first step, of the rest
     uint32_t* top;   // [kQ4Tokens]: bits of the largest finite |x|
     float* table;    // per group
     unsigned char* xs;
@@ -551,7 +554,7 @@ struct Q4Shared {
         red = reinterpret_cast<float*>(smem);
         part = red + 2 * kQ4Warps * (16 * 8 * NT + kQ4RedPad);
         up = part + (shape.splits > 1 ? 2 * shape.wr * 16 * n : 0);
-        top = reinterpret_cast<uint32_t*>(up + kQ4Tokens);
+        top = reinterpret_cast<uint32_t*>(up + 2 * kQ4Tokens);
         table = reinterpret_cast<float*>(top + kQ4Tokens);
         xs = reinterpret_cast<unsigned char*>(table + shape.blocks * 8 * table_floats);
     }
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_halves_kernel(const Q4Mat
         }
     };
     if (threadIdx.x < kQ4Tokens) {
-        sh.up[threadIdx.x] = 1.0f;
+        sh.up[threadIdx.x] = sh.up[kQ4Tokens + threadIdx.x] = 1.0f;
         sh.top[threadIdx.x] = 0;
     }
     if constexpr (kSums) {  // columns that nobody reads
@@ -659,7 +662,8 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_halves_kernel(const Q4Mat
             for (uint32_t i = threadIdx.x; i < all; i += kQ4MulThreads) {
                 const uint4 a = *hi_slot(x), b = *lo_slot(x);
                 const uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-                const uint32_t field = scale_to(sh.top[x.token], 14);
+                // one step is enough: at 2^127 the parts' multiples of 2^-24 are finer than binary32's of 2^-149
+                const uint32_t field = first_step(scale_to(sh.top[x.token], 14));
                 const float scale = power(field);
                 if (x.at == 0) sh.up[x.token] = inverse_power(field);
                 float sum = 0.0f;
@@ -763,7 +767,7 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4Mat
         return sh.table[(group >> 1) * 2 * kTable + (col >> 1) * (kSums ? 8 : 4) + (group & 1u) * 2 + (col & 1u)];
     };
     if (threadIdx.x < kQ4Tokens) {
-        sh.up[threadIdx.x] = 1.0f;
+        sh.up[threadIdx.x] = sh.up[kQ4Tokens + threadIdx.x] = 1.0f;
         sh.top[threadIdx.x] = 0;
     }
     for (uint32_t i = threadIdx.x; i < w.here * 8 * (8 - cols); i += kQ4MulThreads) {  // columns that nobody reads
@@ -821,17 +825,22 @@ __global__ void __launch_bounds__(kQ4MulThreads, 1) q4_digits_kernel(const Q4Mat
                 y[2 * e + 1] = bitsf(b.y);
             }
             const uint32_t largest = sh.top[x.token], field = largest >= kInfinity ? 127u : scale_to(largest, 29);
-            const float scale = power(field);
+            const float scale = power(first_step(field)), rest = power(rest_step(field));
             uint32_t d[8];
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int X = __float2int_rn(y[e] * scale);
+                float z = y[e] * scale;
+                if constexpr (F32) z *= rest;  // binary16 columns never need it
+                const int X = __float2int_rn(z);
                 if constexpr (kSums) sum += (float)X;
                 d[e] = ((uint32_t)X + 0x00808080u) ^ 0x00808080u;  // four balanced digits
             }
             // an infinity or NaN takes the whole column
-            if (x.at == 0) sh.up[x.token] = largest >= kInfinity ? bitsf(0x7fc00000u) : inverse_power(field);
+            if (x.at == 0) {
+                sh.up[x.token] = largest >= kInfinity ? bitsf(0x7fc00000u) : inverse_power(first_step(field));
+                sh.up[kQ4Tokens + x.token] = inverse_power(rest_step(field));
+            }
             // bytes i of the columns 0, 2, 1, 3 and 4, 6, 5, 7
             uint32_t digit[4][2];
 #pragma unroll
@@ -921,7 +930,7 @@ uint64_t q4_shared_bytes(const Q4Shape& s, const Q4MatvecPlan& p) {
     const bool digits = q4_by_digits(p), sums = p.code != kDtypeQ4_0;
     const uint64_t parts = digits ? 4 : p.x_f16 ? 1 : 2, cols = (p.n * parts + 7) / 8 * 8;
     const uint64_t table = digits ? (sums ? 16 : 8) : sums ? cols : 0;
-    return 2 * kQ4Warps * (16 * cols + kQ4RedPad) * 4 + (s.splits > 1 ? 2 * s.wr * 16 * p.n * 4 : 0) + kQ4Tokens * 8 +
+    return 2 * kQ4Warps * (16 * cols + kQ4RedPad) * 4 + (s.splits > 1 ? 2 * s.wr * 16 * p.n * 4 : 0) + kQ4Tokens * 12 +
            s.blocks * 8 * table * 4 + p.n * parts * s.x_row;
 }
 

@@ -111,6 +111,15 @@ def test_activations_of_any_size(emel, kern, size):
     check(emel, kern, "q4_0", 512, 40, 2, values=lambda rng, s: rng.standard_normal(s) * size)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("n", [1, 2, 3])
+@pytest.mark.parametrize("size", [1e-32, 1e-34, 1e-37, 1e-40])
+def test_activations_near_the_smallest_numbers(emel, kern, fmt, n, size):
+    """Down to subnormal columns, which have fewer bits themselves, and subnormal results: every sum has 2^-23
+    of its parts at least, far above half of 2^-149."""
+    check(emel, kern, fmt, 512, 40, n, values=lambda rng, s: rng.standard_normal(s) * size)
+
+
 def test_not_finite_activations_stay_in_their_column(emel, kern):
     rng = np.random.default_rng(3)
     raw = dh.q4_random(rng, "q4_1", 30, 256)
