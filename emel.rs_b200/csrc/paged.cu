@@ -185,9 +185,9 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan 
 // other.  A binary32 query keeps its precision by parts
 // instead: 8 heads, rows 0..7 the parts of highest weight, rows 8..15 the
 // next ones -- binary16 caches: 2 parts of 11 bits, of the query divided by
-// the power of two that brings its largest element into [1, 2), and of the
+// the power of two that brings its largest finite element into [1, 2), and of the
 // weights; bfloat16 caches: 3 parts of 8 bits, the last one in a second
-// operand.  The tensor pipe has room for that: the added products cost nothing
+// operand, of queries below 2^-40 brought up to that.  The tensor pipe has room for that: the added products cost nothing
 // in time.
 constexpr int kAttnWarps = 4;                      // that compute
 constexpr int kAttnConsumers = kAttnWarps * 32;
@@ -276,6 +276,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&h);
     }
+}
+
+// The smallest 16-bit number, with x's sign.
+template <typename C>
+__device__ __forceinline__ C smallest(float x) {
+    const uint16_t bits = (uint16_t)(fbits(x) >> 31 << 15 | 1u);
+    return *reinterpret_cast<const C*>(&bits);
 }
 
 // What is left of x after its 16-bit rounding (0 for what is not finite: the
@@ -531,25 +538,29 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<DP>::kCtas) paged_attn
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) y[c] = there && lane + 32 * c < d ? to_f32(x[i][c]) : 0.0f;
             float up = 1.0f, down = 1.0f;
-            if constexpr (PARTS == 2) {
-                float big = 0.0f;
+            if constexpr (PARTS >= 2) {
+                float big = 0.0f;  // the largest finite one; a subnormal counts as 2^-126
 #pragma unroll
-                for (int c = 0; c < DP / 32; ++c) big = fmaxf(big, fabsf(y[c]));
-                const uint32_t bits = __reduce_max_sync(0xffffffffu, fbits(big));
-                const int e = (int)(bits >> 23) - 127;
-                if (e < 128 && e >= -126) {
-                    down = bitsf((uint32_t)(e < 127 ? 127 - e : 1) << 23);
-                    up = 1.0f / down;
-                }
+                for (int c = 0; c < DP / 32; ++c) big = fmaxf(big, fabsf(y[c]) < INFINITY ? fabsf(y[c]) : 0.0f);
+                const uint32_t field = __reduce_max_sync(0xffffffffu, fbits(big)) >> 23;
+                const int e = field > 0 ? (int)field - 127 : -126;
+                // bfloat16 parts lose bits below 2^-133 only, and round the largest binary32 numbers to infinity
+                const int by = PARTS == 2 ? (e < 127 ? -e : -126) : e < -40 ? -40 - e : e == 127 ? -1 : 0;
+                down = bitsf((uint32_t)(127 + by) << 23);
+                up = bitsf((uint32_t)(127 - by) << 23);
             }
-            if (lane == 0) q_scale[r] = p.scale * kLog2e * up;
+            if (lane == 0) q_scale[r] = p.scale * up * kLog2e;
 #pragma unroll
             for (int c = 0; c < DP / 32; ++c) {
                 const uint32_t col = lane + 32 * c;
                 const float z = y[c] * down;
-                *reinterpret_cast<C*>(q_tile + r * kRow + col * 2) = from_f32<C>(z);
+                C first = from_f32<C>(z);
+                // what rounds to 0 keeps its sign for a key that is infinite (0 would make a NaN of it); the
+                // next part takes the smallest number back
+                if (PARTS >= 2 && y[c] != 0.0f && to_f32(first) == 0.0f) first = smallest<C>(y[c]);
+                *reinterpret_cast<C*>(q_tile + r * kRow + col * 2) = first;
                 if constexpr (PARTS >= 2) {
-                    const float rest = rest_of<C>(z);
+                    const float left = z - to_f32(first), rest = fabsf(left) < INFINITY ? left : 0.0f;
                     *reinterpret_cast<C*>(q_tile + (8 + r) * kRow + col * 2) = from_f32<C>(rest);
                     if constexpr (PARTS == 3)
                         *reinterpret_cast<C*>(q_tile + (16 + r) * kRow + col * 2) = from_f32<C>(rest_of<C>(rest));

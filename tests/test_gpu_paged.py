@@ -172,6 +172,56 @@ def test_infinite_scores(emel, kern):
     assert np.isnan(got[2]).all()
 
 
+@pytest.mark.parametrize("kvkind", ["f16", "bf16"])
+@pytest.mark.parametrize("size,scale", [(1e-39, 2e38), (1e-36, 1e35), (1e-30, 1e29), (1e37, 1e-38)])
+def test_queries_of_any_size(emel, kern, kvkind, size, scale):
+    """From subnormal queries to the largest: the scale brings the scores back."""
+    q, k, v, table, lengths, out = setup(emel, kern.ctx, 11, [70, 9], 1, 4, 32, 16, "f32", kvkind)
+    q = dh.Dev(emel, kern.ctx, q.values * size, "f32")
+    check(emel, kern, (q, k, v, table, lengths, out), scale=scale)
+
+
+@pytest.mark.parametrize("kvkind", ["f16", "bf16"])
+@pytest.mark.parametrize("q,k,scale", [
+    ([1.0, 1e-9, 0.5], [1.0, -np.inf, 1.0], 0.5),     # too small for a 16-bit part, and its key is infinite: -inf, not NaN
+    ([1.0, 1e-41, 0.5], [1.0, -np.inf, 1.0], 0.5),
+    ([1e30, -1e-9, 0.5], [1.0, np.inf, 1.0], 1e-30),
+    ([3.4e38, 0.0, 0.0], [-1e-30, 0.0, 0.0], 1e-38),  # above the largest bfloat16 number
+    ([np.finfo(np.float32).max, 0.0, 0.0], [-1e-5, 0.0, 0.0], 1e-38),
+    ([1e-3, 0.0, 0.0], [-65504.0, 0.0, 0.0], 0.1)])
+def test_parts_of_queries_beside_infinities_and_at_the_ends(emel, kern, kvkind, q, k, scale):
+    """One row of few products: off by (16 + 16) 2^-23 of its values, and by (3 + 16) 2^-23 of scores up to 1 twice."""
+    ctx, d, page = kern.ctx, 16, 8
+    qq, kk = np.zeros((1, 1, d)), np.zeros((1, page, 1, d))
+    qq[0, 0, :3] = q
+    kk[0, :, 0, :3] = [0.25 if x > 0 else 0.0 for x in q]
+    kk[0, 3, 0, :3] = k
+    qd, kd = dh.Dev(emel, ctx, qq, "f32"), dh.Dev(emel, ctx, kk, kvkind)
+    vd = dh.Dev(emel, ctx, np.random.default_rng(1).standard_normal(kk.shape), kvkind)
+    table, lengths, out = dh.Dev(emel, ctx, [[0]], "i32"), dh.Dev(emel, ctx, [page], "i32"), dh.Dev(emel, ctx, qq, "f32")
+    assert kern.process_event(emel.OpPagedAttn(qd.c(), kd.c(), vd.c(), table.c(), lengths.c(), out.c(), scale)) == 0
+    s = np.array([sum(a * b for a, b in zip(qd.values[0, 0], row) if a and b) for row in kd.values[0, :, 0]]) * scale
+    p = np.exp(s - s.max())
+    want = p @ vd.values[0, :, 0] / p.sum()
+    most = np.abs(s[np.isfinite(s)]).max()
+    assert np.abs(out.read()[0, 0] - want).max() <= np.abs(vd.values).max() * 2.0 ** -23 * (32 + 2 * 19 * most)
+
+
+@pytest.mark.parametrize("kvkind", ["f16", "bf16"])
+def test_infinite_queries(emel, kern, kvkind):
+    """Every score is -inf, whatever large numbers stand beside the infinity: zeros."""
+    ctx = kern.ctx
+    q = np.zeros((1, 1, 16))
+    q[0, 0, :3] = [np.inf, 1e6, -1e6]
+    k = np.zeros((1, 8, 1, 16))
+    k[..., :3] = [-0.5, 1.0, 1.0]
+    k[..., 3:] = 1.0
+    qd, kd, vd = dh.Dev(emel, ctx, q, "f32"), dh.Dev(emel, ctx, k, kvkind), dh.Dev(emel, ctx, k, kvkind)
+    table, lengths, out = dh.Dev(emel, ctx, [[0]], "i32"), dh.Dev(emel, ctx, [8], "i32"), dh.Dev(emel, ctx, q + 7.0, "f32")
+    assert kern.process_event(emel.OpPagedAttn(qd.c(), kd.c(), vd.c(), table.c(), lengths.c(), out.c())) == 0
+    assert (out.read() == 0).all()
+
+
 @pytest.mark.parametrize("kind", ["f16", "bf16"])
 @pytest.mark.parametrize("kvh,rep,d", [(2, 1, 8), (1, 4, 16), (1, 9, 8), (1, 17, 16)])
 def test_16_bit_queries_round_only_the_result(emel, kern, kind, kvh, rep, d):
