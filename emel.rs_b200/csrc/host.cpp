@@ -1816,7 +1816,7 @@ emel_cuda_status emel_cuda_paged_attn(emel_cuda_context* ctx, void* stream, cons
     if (!unit_rows(query, cq) || !unit_rows(dst, cd)) return EMEL_CUDA_INVALID_LAYOUT;
     const uint64_t d = key_cache->ne[0], kv_heads = key_cache->ne[1], heads = query->ne[1], batch = query->ne[2];
     if (!same_ne(query, dst) || query->ne[0] != d || query->ne[3] != 1 || heads % kv_heads != 0 ||
-        heads > 0x7fffffffull || block_table->ne[1] != batch || !vector_shape(lengths, batch))
+        heads > 0x7fffffffull || batch > emel::kCountedMost || block_table->ne[1] != batch || !vector_shape(lengths, batch))
         return EMEL_CUDA_SHAPE_MISMATCH;
     float scale = 1.0f / std::sqrt((float)d);
     if (options != nullptr && options->has_scale) scale = options->scale;
@@ -1961,7 +1961,8 @@ emel_cuda_status emel_cuda_logits_adjust(emel_cuda_context* ctx, void* stream, c
         return v->ne[0] == cols && (v->ne[1] == rows || (shared_ok && v->ne[1] == 1)) && v->ne[2] == 1 && v->ne[3] == 1;
     };
     if (!same_ne(src, dst) || src->ne[2] != 1 || src->ne[3] != 1 ||
-        (past && (!table(history, history->ne[0], false) || !vector_shape(history_lengths, rows) ||
+        (past && (history->ne[0] > emel::kCountedMost || !table(history, history->ne[0], false) ||
+                  !vector_shape(history_lengths, rows) ||
                   !table(penalties, 3, true))) ||
         (bias != nullptr && !table(bias, vocab, true)) || (allowed != nullptr && !table(allowed, words, true)))
         return EMEL_CUDA_SHAPE_MISMATCH;
@@ -1971,7 +1972,7 @@ emel_cuda_status emel_cuda_logits_adjust(emel_cuda_context* ctx, void* stream, c
                   views_overlap(dst, cd, penalties, cp))) ||
         (bias != nullptr && views_overlap(dst, cd, bias, cb)) ||
         (allowed != nullptr && views_overlap(dst, cd, allowed, ca)) ||
-        vocab > 0x7fff0000ull || emel::logits_blocks(vocab, rows) > 0x7fffffffull)
+        vocab > emel::kCountedMost || emel::logits_blocks(vocab, rows) > 0x7fffffffull)
         return EMEL_CUDA_INVALID_ARGUMENT;
     emel::LogitsPlan p{};
     p.src = static_cast<const char*>(src->data);

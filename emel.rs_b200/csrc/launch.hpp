@@ -209,6 +209,9 @@ cudaError_t launch_diag(const LaunchEnv& env, const DiagPlan& plan, int mode);
 // Paged key/value cache (paged.cu).  Caches are [d, kv_heads, page_size,
 // pages] with byte strides; the block table is [pages of a sequence, sequence].
 constexpr int kPagedMaxD = 256;
+// Sequences of the attention and ids of a row's history are counted in signed 32
+// bits, by steps of far less than 2^16.
+constexpr uint64_t kCountedMost = 0x7fff0000ull;
 
 struct PagedAppendPlan {
     const char* key;        // [d, kv_heads, count], byte strides, unit element stride in dim 0

@@ -794,8 +794,8 @@ EMEL_CUDA_API emel_cuda_status emel_cuda_paged_kv_append(emel_cuda_context* ctx,
  * is taken as the table's and rejected (see above); tokens of a rejected page
  * are left out.  dst may not overlap an input.
  * options NULL: scale 1 / sqrt(d), no window.
- * Statuses: INVALID_VIEW, INVALID_LAYOUT, SHAPE_MISMATCH, INVALID_PARAMETERS
- * (scale not finite or not positive), INVALID_ARGUMENT (null context, an
+ * Statuses: INVALID_VIEW, INVALID_LAYOUT, SHAPE_MISMATCH (more than 2^31 - 2^16
+ * sequences among them), INVALID_PARAMETERS (scale not finite or not positive), INVALID_ARGUMENT (null context, an
  * overlapping dst).  Uses the context's workspace: calls of one
  * context must not overlap on the GPU. */
 typedef struct emel_paged_attn_options {
@@ -860,9 +860,10 @@ EMEL_CUDA_API emel_cuda_status emel_cuda_mul_mat_q4(emel_cuda_context* ctx, void
  *   allowed (I32 [ceil(vocab / 32), rows] or [.., 1], unit rows; nullable):
  *     v = -inf where bit i % 32 of word i / 32 is 0, whatever v was.
  * Statuses: INVALID_VIEW (also a partial history), INVALID_LAYOUT,
- * SHAPE_MISMATCH, INVALID_ARGUMENT (null context, dst overlapping an input
- * otherwise than as src itself, more than 2^31 - 2^16 logits in a row or 2^31 - 1
- * pieces of 4096 logits). */
+ * SHAPE_MISMATCH (a capacity of more than 2^31 - 2^16 ids among them),
+ * INVALID_ARGUMENT (null context, dst overlapping an input otherwise than as
+ * src itself, more than 2^31 - 2^16 logits in a row or 2^31 - 1 pieces of 4096
+ * logits). */
 EMEL_CUDA_API emel_cuda_status emel_cuda_logits_adjust(emel_cuda_context* ctx, void* stream,
                                                        const emel_tensor_view* src, const emel_tensor_view* history,
                                                        const emel_tensor_view* history_lengths,

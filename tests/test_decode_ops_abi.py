@@ -76,6 +76,16 @@ def test_attention(emel):
     assert attn(emel, opts=emel.CPagedAttnOptions(0.0, 0, 7, 1)) == PARAMS
 
 
+def test_counts_that_would_wrap_are_refused(emel):
+    """Sequences and ids of a history are walked with signed 32-bit counters, in steps of up to a few thousand."""
+    for n, st in (((1 << 31) - (1 << 16), OK), ((1 << 31) - (1 << 16) + 1, SHAPE), ((1 << 31) - 1, SHAPE)):
+        q = ((1, 1, n), "f16")
+        cache = ((1, 1, 1, 1), "f16")
+        assert attn(emel, q=q, out=(q[0], "f16", {"data": 1 << 46}), k=cache, v=cache, table=((1, n), "i32"),
+                    lengths=((n,), "i32")) == st
+        assert logits(emel, history=((n, 4), "i32")) == st
+
+
 def test_events_take_views_and_keep_their_fields(emel):
     v = view(emel, 0, (64, 8, 3), "f32")
     with pytest.raises(TypeError):
