@@ -1154,6 +1154,7 @@ class Q4Weights:
 
     def free(self):
         self.buffer.free()
+        self.c.data = None  # events that still name these weights are refused
 
 
 @dataclass(frozen=True)

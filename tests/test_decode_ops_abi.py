@@ -230,3 +230,44 @@ def test_overlaps_are_refused(emel):
     assert lib.emel_cuda_logits_adjust(h, None, B(src), None, None, None, B(bias), None, B(src)) == OK
     ctx.synchronize()
     buf.free()
+
+
+class HostOnly:
+    """A context whose memory and layout kernel are stand-ins: host logic without a GPU."""
+
+    def __init__(self, emel):
+        self.handle, self.freed, real = None, [], emel.lib()
+
+        class Lib:
+            def __getattr__(_, name):
+                return getattr(real, name)
+
+            def emel_cuda_malloc(_, ctx, n, out):
+                out._obj.value = FAR
+                return 0
+
+            def emel_cuda_free(_, ctx, at):
+                self.freed.append(at)
+                return 0
+
+            def emel_cuda_q4_pack(_, ctx, stream, src, data, n, out):
+                w, v = out._obj, src._obj
+                w.data, w.bytes, w.k, w.rows, w.dtype, w.reserved = data.value, n, v.ne[0], v.ne[1], v.dtype, 0
+                return 0
+
+        self._lib = Lib()
+
+
+def test_weights_that_were_freed_are_refused(emel):
+    """Their events keep the handle: it names no memory any more."""
+    ctx = HostOnly(emel)
+    src = view(emel, 3, (64, 16, 1, 1), "i32", nb=[1, 36, 576, 576], storage=576)
+    src.dtype = dh.CODES["q4_0"]
+    w = emel.Q4Weights(ctx, src)
+    event = emel.OpMulMatQ4(w, view(emel, 1, (64, 2), "f32"), view(emel, 2, (16, 2), "f32"))
+    assert event.dispatch(ctx, None) == OK
+    w.free()
+    assert ctx.freed == [FAR]
+    assert event.dispatch(ctx, None) == VIEW
+    w.free()
+    assert ctx.freed == [FAR]
