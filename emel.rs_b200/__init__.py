@@ -1128,6 +1128,8 @@ class OpPagedAttn(_StepEvent):
 
     def __post_init__(self):
         super().__post_init__()
+        if not 0 <= self.window < 1 << 32:
+            raise ValueError(f"window is {self.window}, not a number of tokens below 2^32 (0: all)")
         opts = CPagedAttnOptions(self.scale or 0.0, self.scale is not None, self.window, 0)
         object.__setattr__(self, "_options", (opts, ctypes.addressof(opts)))
 

@@ -232,6 +232,20 @@ def test_overlaps_are_refused(emel):
     buf.free()
 
 
+def test_windows_that_do_not_fit_are_refused(emel):
+    """They would be taken modulo 2^32, and a window of 2^32 for none."""
+    views = [view(emel, i, ne, kind) for i, (ne, kind) in enumerate(
+        [((64, 8, 3), "f32"), ((64, 2, 16, 10), "f16"), ((64, 2, 16, 10), "f16"), ((5, 3), "i32"), ((3,), "i32"), ((64, 8, 3), "f32")])]
+    ctx = type("Ctx", (), {"_lib": emel.lib(), "handle": None})
+    for window in (-1, 1 << 32, -(1 << 40)):
+        with pytest.raises(ValueError, match="window"):
+            emel.OpPagedAttn(*views, window=window)
+    with pytest.raises(TypeError):
+        emel.OpPagedAttn(*views, window=1.5)
+    for window in (0, 1, (1 << 32) - 1, np.int64(7)):
+        assert emel.OpPagedAttn(*views, window=window).dispatch(ctx, None) == OK
+
+
 class HostOnly:
     """A context whose memory and layout kernel are stand-ins: host logic without a GPU."""
 
