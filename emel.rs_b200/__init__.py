@@ -1087,6 +1087,14 @@ class _StepEvent(Event):
         fixed = all(v is None or isinstance(v, CView) for v in views)
         object.__setattr__(self, "_at", tuple(v and ctypes.addressof(v) for v in views) if fixed else None)
 
+    def __getstate__(self):  # a copy takes the fields and finds the addresses of its own
+        return {name: getattr(self, name) for name in self.__dataclass_fields__}
+
+    def __setstate__(self, state):
+        for name, value in state.items():
+            object.__setattr__(self, name, value)
+        self.__post_init__()
+
     def _args(self):
         if self._at is not None:
             return self._at

@@ -246,6 +246,29 @@ def test_windows_that_do_not_fit_are_refused(emel):
         assert emel.OpPagedAttn(*views, window=window).dispatch(ctx, None) == OK
 
 
+@pytest.mark.parametrize("how", ["copy", "deepcopy", "pickle", "replace"])
+def test_copies_of_an_event_stand_on_their_own(emel, how):
+    """An event keeps the addresses of its options and views; a copy's are those of the copy's own."""
+    import copy
+    import dataclasses
+    import pickle
+    layout = lambda ne, kind: emel.Layout.contiguous(emel.DType(dh.CODES[kind]), list(ne) + [1] * (4 - len(ne)))  # noqa: E731
+    views = [emel.TensorView(FAR * (i + 1), 1 << 20, layout(ne, kind)) for i, (ne, kind) in enumerate(
+        [((64, 8, 3), "f32"), ((64, 2, 16, 10), "f16"), ((64, 2, 16, 10), "f16"), ((5, 3), "i32"), ((3,), "i32"), ((64, 8, 3), "f32")])]
+    event = emel.OpPagedAttn(*views, scale=0.25, window=9)
+    made = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda e: pickle.loads(pickle.dumps(e)),
+            "replace": lambda e: dataclasses.replace(e, window=9)}[how](event)
+    assert made == event
+    options, at = made._options
+    assert at == ctypes.addressof(options) and (options.scale, options.window) == (0.25, 9)
+    if how in ("deepcopy", "pickle", "replace"):
+        assert options is not event._options[0]
+    held = emel.OpLogitsAdjust(views[0].c(), views[5].c())
+    if how in ("copy", "replace"):  # a CView is an address: Python does not copy it more deeply
+        other = copy.copy(held) if how == "copy" else dataclasses.replace(held, dst=views[1].c())
+        assert other._at == tuple(v and ctypes.addressof(v) for v in (getattr(other, n) for n in other.VIEWS))
+
+
 class HostOnly:
     """A context whose memory and layout kernel are stand-ins: host logic without a GPU."""
 
