@@ -119,16 +119,20 @@ class Decoder:
             raise RuntimeError(f"{type(event).__name__}: {status.name} ({self.ctx.last_error})")
 
     # -- one step -----------------------------------------------------------
-    def reserve(self):
-        """Counts one more token for every sequence, and gives a page to those that begin one."""
+    def beginning(self):
+        """The sequences whose next token begins a page; raises, with nothing changed, when it has no place."""
         c = self.c
         if int(self.lengths.max()) >= c.capacity:
             raise RuntimeError("a sequence has reached the capacity of its table")
-        for b in range(self.batch):
-            if self.lengths[b] % c.page == 0:
-                if not self.free_pages:
-                    raise RuntimeError("the cache has no free page")
-                self.table[b, self.lengths[b] // c.page] = self.free_pages.pop()
+        begin = np.flatnonzero(self.lengths % c.page == 0)
+        if len(begin) > len(self.free_pages):
+            raise RuntimeError("the cache has no free page")
+        return begin
+
+    def reserve(self, begin):
+        """Counts one more token for every sequence, and gives a page to those that begin one."""
+        for b in begin:
+            self.table[b, self.lengths[b] // self.c.page] = self.free_pages.pop()
         self.put("positions", self.lengths)
         self.lengths += 1
         self.put("lengths", self.lengths)
@@ -180,8 +184,9 @@ class Decoder:
     def step(self, tokens, graph=None):
         """Feeds one token per sequence; returns the tokens chosen next."""
         tokens = np.ascontiguousarray(tokens, I32)
+        begin = self.beginning()
         self.remember(tokens)
-        self.reserve()
+        self.reserve(begin)
         self.put("tokens", tokens)
         if graph is None:
             self.enqueue()

@@ -116,3 +116,36 @@ def test_a_cache_without_pages_says_so(emel):
         model.step(np.zeros(2, np.int32))
     with pytest.raises(RuntimeError, match="no free page"):
         model.step(np.zeros(2, np.int32))
+
+
+def state(model):
+    return [x.copy() for x in (model.table, model.lengths, model.history)] + [sorted(model.free_pages)]
+
+
+def test_a_refused_step_changes_nothing_and_loses_no_page(emel):
+    import decode_step as ex
+    c = ex.Config(pages=3)
+    model = ex.Decoder(emel, c, ex.random_weights(c, 2), 2)
+    for _ in range(16):
+        model.step(np.zeros(2, np.int32))
+    before = state(model)
+    for _ in range(2):  # two pages are needed, one is free
+        with pytest.raises(RuntimeError, match="no free page"):
+            model.step(np.ones(2, np.int32))
+        assert all(np.array_equal(a, b) for a, b in zip(before, state(model)))
+    model.free_pages.append(int(model.table[0, 0]))  # the first sequence ends, another takes its place
+    model.table[0], model.lengths[0] = -1, 0
+    model.step(np.ones(2, np.int32))
+    assert sorted(model.free_pages + list(model.table[model.table >= 0])) == [0, 1, 2]
+
+
+def test_a_full_table_says_so(emel):
+    import decode_step as ex
+    c = ex.Config(capacity=32)
+    model = ex.Decoder(emel, c, ex.random_weights(c, 2), 2)
+    for _ in range(32):
+        model.step(np.zeros(2, np.int32))
+    before = state(model)
+    with pytest.raises(RuntimeError, match="capacity"):
+        model.step(np.zeros(2, np.int32))
+    assert all(np.array_equal(a, b) for a, b in zip(before, state(model)))
