@@ -84,7 +84,7 @@ class Decoder:
         for i in range(c.layers):
             for kv in "kv":
                 self.put(f"cache.{kv}{i}", np.zeros(c.pages * c.page * c.kv_heads * hd, np.float16))
-        self.columns = c.capacity // c.page
+        self.columns = -(-c.capacity // c.page)
         self.table = np.full((b, self.columns), -1, I32)
         self.free_pages = list(range(c.pages))[::-1]
         self.lengths = np.zeros(b, I32)

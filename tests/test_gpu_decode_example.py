@@ -149,3 +149,13 @@ def test_a_full_table_says_so(emel):
     with pytest.raises(RuntimeError, match="capacity"):
         model.step(np.zeros(2, np.int32))
     assert all(np.array_equal(a, b) for a, b in zip(before, state(model)))
+
+
+def test_a_capacity_that_ends_inside_a_page(emel):
+    import decode_step as ex
+    c = ex.Config(capacity=20)
+    model = ex.Decoder(emel, c, ex.random_weights(c, 2), 2)
+    for _ in range(20):
+        model.step(np.zeros(2, np.int32))
+    with pytest.raises(RuntimeError, match="capacity"):
+        model.step(np.zeros(2, np.int32))
