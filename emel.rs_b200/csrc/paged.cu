@@ -149,11 +149,14 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(PagedAppendPlan 
 //
 //     s_t = scale q . k_t,  m = max s,  out = sum e^(s - m) v / sum e^(s - m)
 //
-// Every key and value is read once from HBM, and that is what bounds the
-// kernel: 4 flops a cached element and head are far under the tensor rate.
+// Every key and value is read once from HBM for each unit, and that is what bounds
+// the kernel: 4 flops a cached element and head are far under the tensor rate.
 //
-// Work.  A unit is one key/value head of one sequence with up to HPU of the
-// query heads that share it; its tokens form tiles of 64.  All tiles of all
+// Work.  A unit is one key/value head of one sequence with up to HPU (8 of binary32,
+// 16 of 16 bits) of the query heads that share it; its tokens form tiles of 64.  More
+// heads are more units, which read the same tiles again: 64 sequences of 8191 tokens
+// over one head of 128, 269 MB, take 56 us with 8 binary32 query heads over binary16,
+// 97 with 9, 180 with 32; in bfloat16 62 us with 16, 102 with 17.  All tiles of all
 // units, in order, are cut into equal runs, one for each CTA, so a batch of
 // any mixture of lengths loads every SM alike; a unit cut between CTAs leaves
 // its pieces (m, l, o) in the workspace, and the CTA that finishes last (a

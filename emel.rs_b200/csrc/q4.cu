@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackPlan p) {
 // One or two tokens (q4_digits_kernel, m16n8k32 on 8-bit integers): a mask
 // leaves four quants of a word, a shift and a mask the other four, three
 // instructions for 8 weights.  A token is x 2^e rounded to an integer of 31
-// bits (e per token and CTA: the largest finite |x| in [2^29, 2^30)), and its four
+// bits (e per token and CTA: the largest finite |x| in [2^29, 2^30), subnormals below), and its four
 // balanced digits to the base 256 are four columns.  A group's integer sum is exact; it
 // comes out of the product on top of the bits of 1.5 2^23, so that one
 // addition, of minus that and 8 times the digits' sum, makes sum((q - 8) digit) a
@@ -140,7 +140,9 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackPlan p) {
 //
 // More tokens (q4_halves_kernel, m16n8k16 on binary16): a mask leaves the bits
 // of 1024 + q or, four bits higher up, of 1024 + 16 q, one subtraction or
-// multiply-add makes q - 8 of them, exactly; nine instructions for 8 weights.
+// multiply-add makes q - 8 of them, exactly (the conversion by 1024's exponent as
+// published for mixed-precision products: Kim, Henry, Fahim and Awadalla, "Who Says
+// Elephants Can't Run", 2022); nine instructions for 8 weights.
 // (The masked bits alone, as the subnormals q 2^-24, would take five, but
 // their products came out with errors of 2^-17.)  A binary16
 // token is one column as it is; a binary32 token is two, x 2^e = hi + lo, both
@@ -159,7 +161,8 @@ __global__ void __launch_bounds__(kQ4Threads) q4_pack_kernel(Q4PackPlan p) {
 //
 // One token, 4096 columns: 151936 rows of Q4_0, 350 MB, bound by HBM, 57 us in short
 // runs, 6.1 TB/s, and 65 us where a long run meets the power limit; 14336 rows of
-// Q4_K, 33 MB, 11.4 us, of which about 4 are start and preparation.  Eight binary32 tokens,
+// Q4_K, 33 MB, 11.4 us, of which about 4 are start and preparation; whole rounds of
+// tiles leave 112 of 148 SMs with work there.  Eight binary32 tokens,
 // 11007 rows of Q4_1: 19.0 us, bound by instructions; binary16 tokens 13.0 us.
 constexpr int kQ4Warps = 16;
 constexpr int kQ4MulThreads = kQ4Warps * 32;

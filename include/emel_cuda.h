@@ -767,7 +767,7 @@ EMEL_CUDA_API emel_cuda_status emel_gguf_upload(emel_cuda_context* ctx, void* st
  * NULL: of sequence i, and count is the table's number of sequences).  A
  * negative position skips its row, a rejected one writes nothing; F32 is
  * rounded once, to nearest even.  No two rows may name the same position of
- * one sequence.
+ * one sequence, and key and value may not hold places that the call writes.
  * Statuses: INVALID_VIEW, INVALID_LAYOUT, SHAPE_MISMATCH, INVALID_ARGUMENT
  * (null context). */
 EMEL_CUDA_API emel_cuda_status emel_cuda_paged_kv_append(emel_cuda_context* ctx, void* stream,
@@ -784,19 +784,20 @@ EMEL_CUDA_API emel_cuda_status emel_cuda_paged_kv_append(emel_cuda_context* ctx,
  * key/value head h / (heads / kv_heads); lengths is I32 [batch].  With
  * n = lengths[b] and t over [window ? max(0, n - window) : 0, n):
  *     s_t = scale * q . k_t,   dst = sum exp(s_t - max s) v_t / sum exp(s_t - max s)
- * A sequence without tokens (n <= 0) gives zeros, and so does one whose every
+ * A sequence without tokens (n <= 0; nothing is rejected) gives zeros, and so does one whose every
  * score is -inf; a NaN or +inf score, or a value that is not finite, gives
  * what is not finite.  Whatever lies in the cache beyond the n tokens (or before
  * the window) has no effect, NaN and infinities included.  Scores, weights'
  * sums and products are binary32, rounded once to dst's type; a weight counts
  * to within 2^-21 of its own value (16-bit queries over BF16: 2^-17) or 2^-32 of
- * the largest one's, whichever is more.  A length beyond the table
+ * the largest one's, whichever is more.  scale times the largest finite |q| has
+ * to stay below 2^127.  A length beyond the table
  * is taken as the table's and rejected (see above); tokens of a rejected page
  * are left out.  dst may not overlap an input.
  * options NULL: scale 1 / sqrt(d), no window.
  * Statuses: INVALID_VIEW, INVALID_LAYOUT, SHAPE_MISMATCH (more than 2^31 - 2^16
- * sequences among them), INVALID_PARAMETERS (scale not finite or not positive), INVALID_ARGUMENT (null context, an
- * overlapping dst).  Uses the context's workspace: calls of one
+ * sequences among them), INVALID_PARAMETERS (scale not finite or not positive),
+ * INVALID_ARGUMENT (null context, an overlapping dst).  Uses the context's workspace: calls of one
  * context must not overlap on the GPU. */
 typedef struct emel_paged_attn_options {
     float scale;
@@ -822,8 +823,8 @@ typedef struct emel_q4_weights {
     uint32_t reserved; /* 0 */
 } emel_q4_weights;
 /* Bytes of the packed form of `rows` rows of `k` weights (k a multiple of 32,
- * or 256 for Q4_K): the source's size, rounded up to tiles of 16 rows and
- * 64 columns (Q4_K: and 3 % more).  INVALID_ARGUMENT for anything else. */
+ * or 256 for Q4_K): ceil(rows / 16) * (512 ceil(k / 64) + s ceil(k / 256)), s = 256
+ * (Q4_0), 512 (Q4_1) or 320 (Q4_K).  INVALID_ARGUMENT for anything else. */
 EMEL_CUDA_API emel_cuda_status emel_cuda_q4_packed_bytes(uint32_t dtype, uint64_t k, uint64_t rows, uint64_t* bytes);
 /* Lays out src (packed rows as in emel_cuda_mul_mat_argmax_q4_0 /
  * emel_gguf_tensor_view: [k, rows], two-dimensional) into `data` and fills
@@ -833,16 +834,19 @@ EMEL_CUDA_API emel_cuda_status emel_cuda_q4_packed_bytes(uint32_t dtype, uint64_
 EMEL_CUDA_API emel_cuda_status emel_cuda_q4_pack(emel_cuda_context* ctx, void* stream, const emel_tensor_view* src,
                                                  void* data, uint64_t bytes, emel_q4_weights* out);
 /* dst[r, i] = sum over c of w[r, c] * rhs[c, i]: rhs [k, n] F32 or F16, dst
- * [rows, n] F32 or F16, unit rows.  Weights count with their exact values
- * (d (q - 8), d q + m, d s q - e t), products of a group of 32 are summed before
- * they meet its scale, sums are binary32, rounded once to dst's type.  A matrix-vector product for single tokens and
- * small batches: every further 8 columns of rhs read the weights once more.
+ * [rows, n] F32 or F16, unit rows.  Weights are d (q - 8), d q + m or d s q - e t;
+ * the last two count as a (q - 8) + c with c = m + 8 d or 8 d s - e t rounded to
+ * binary32.  Products of a group of 32 are summed before they meet its scale, sums
+ * are binary32, rounded once to dst's type.  A matrix-vector product for single
+ * tokens and small batches: every further 8 columns of rhs read the weights once
+ * more.  Columns are taken 8 at a time, and how many are taken together decides the
+ * order of sums and how activations are split (one or two, or more): the same
+ * column beside others may differ in its last bits, within the bound below.
  * Weights' scales must be finite.  An activation counts to within 2^-23 of its
  * own value or 2^-30 of its column's largest finite one, whichever is more; a
  * column with an infinity or a NaN gives what is not finite.
  * Statuses: INVALID_VIEW (views or weights), INVALID_LAYOUT, SHAPE_MISMATCH
- * (k > 131072 among them),
- * INVALID_ARGUMENT (null context, dst overlapping rhs or the weights). */
+ * (k > 131072 among them), INVALID_ARGUMENT (null context, dst overlapping rhs or the weights). */
 EMEL_CUDA_API emel_cuda_status emel_cuda_mul_mat_q4(emel_cuda_context* ctx, void* stream,
                                                     const emel_q4_weights* weights, const emel_tensor_view* rhs,
                                                     const emel_tensor_view* dst);
